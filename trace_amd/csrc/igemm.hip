@@ -22,7 +22,7 @@
 //     ds_read_b128), the next K-step's LDS-DMA loads in flight during the MFMA block,
 //     one barrier per K-step;
 //   * the same kernel runs plain/batched GEMMs (1 tap, explicit row strides).
-#include "common.h"
+#include "lds_dma.h"
 #include <stdlib.h>
 #include <type_traits>
 
@@ -101,34 +101,8 @@ __device__ __forceinline__ int a_kseg(int wave, int lane) { return (lane & 7) ^ 
 // 4 KiB + one K-step: a halo piece's source pointer walks a whole tap (Crun <= 2048 elements) inside it
 __device__ __attribute__((aligned(256))) const uint4 g_zero_page[264] = {};
 
-typedef const __attribute__((address_space(1))) void* gptr_t;
-typedef __attribute__((address_space(3))) void* lptr_t;
-
-__device__ __forceinline__ void glds16(const void* g, char* lds_wave_base) {
-  __builtin_amdgcn_global_load_lds((gptr_t)g, (lptr_t)lds_wave_base, 16, 0, 0);
-}
-// The same with the NON-TEMPORAL cache policy (aux bit 1 = nt on gfx940+): for operands streamed from HBM exactly once -
-// the weights of the 100352-wide FCs.  A plain load allocates in the memory-side cache and, behind kernels that
-// wrote, pays for the write-back of the dirty lines it evicts: tools/stream_probe.hip reads fc1's 616 MB at 3.4 TB/s
-// with plain loads behind a writer (6.1 TB/s on clean caches) and at 6.8 TB/s with nt loads in either state.
-__device__ __forceinline__ void glds16_nt(const void* g, char* lds_wave_base) {
-  __builtin_amdgcn_global_load_lds((gptr_t)g, (lptr_t)lds_wave_base, 16, 0, 2);
-}
-
 // cout offset (inside a 32-cout group) held by MFMA row `rho` of the even/odd fragment of a pair
 __device__ __forceinline__ int perm_row(int odd, int rho) { return ((rho >> 2) << 3) + (odd << 2) + (rho & 3); }
-
-template <int N> __device__ __forceinline__ void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-
-// The barrier of the LDS rings.  A wave must not ARRIVE with LDS reads still in flight: behind the barrier the other
-// waves refill - by LDS-DMA - the very stage those reads came from (write-after-read).  `__builtin_amdgcn_s_barrier()`
-// alone does not order them: hipcc keeps a stage's last fragment reads in flight across it and waits for them
-// (`s_waitcnt lgkmcnt`) only in front of the MFMAs that it sank below the barrier.  Alone on a CU the reads always win the
-// race against a refill that still has an L2 round trip ahead of it; beside another kernel's workgroups that keep the CU's
-// LDS pipeline busy (a second stream or a forked graph branch) the refill can land first and the MFMA consumes bytes of
-// the NEXT K-step: one wrong 32-position wave column per ~10^5 workgroups, found in round 3 (tools/race_probe.py named the
-// launch, tools/scan_barrier_hazard.py lists every kernel whose assembly had the pattern).
-__device__ __forceinline__ void ring_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Diagnostic build switch (tools/build_variant.py): idle for TRACE_SETTLE_SLEEP x 64 cycles between the barrier that follows
 // a counted wait and the first fragment read of the stage that wait retired.
