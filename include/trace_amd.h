@@ -203,6 +203,7 @@ int trace_clip_to_ndhwc_bf16(const float* in, int N, int C, int T, int H,
 #define TRACE_EPI_POOL_T2 128 /* trace_conv3d_igemm_bf16, 1x1x1 stride-1 convs, even To: the epilogue also applies the
                                * MaxPool3d((2,1,1), stride (2,1,1)) that follows layer1 (resnet3d.py:270, :798): out is
                                * (N,To/2,Ho,Wo,Cout); residual keeps the unpooled shape.  Identical to conv + pool. */
+#define TRACE_EPI_SILU 256   /* z / (1 + exp(-z)): trace_group_norm_act_* only */
 #define TRACE_EPI_WTILED 64  /* trace_gemm_bf16_nt*: Bm is PRE-TILED for weight streaming (N % 128 == 0, K % 64 == 0,
                               * ldb == K): block (n/128, k/64) is 16 KiB contiguous, holding for row r = n % 128 and
                               * 16-byte chunk pc = 0..7 the 8 elements Bm[n][64*(k/64) + 8*(pc ^ (r & 7)) ..] at byte
@@ -537,6 +538,77 @@ int trace_rank_triplets(const float* prd, int P_total, int n_prd, int ld_prd, co
  * Sizes multiples of 16, pointers 16-byte aligned; `pinned` must be device-accessible host memory. */
 int trace_upload_slots(const void* pinned, size_t slot_bytes, unsigned* counter, void* dst, size_t nbytes,
                        trace_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Operators of a training step                                              */
+/* ------------------------------------------------------------------------ */
+
+/* Softmax attention, forward and backward (mmcv's NonLocal3d in its default mode 'embedded_gaussian', call site
+ * lib/i3d/resnet3d.py:289, is one head of it).  bf16 operands, f32 scores / statistics / sums.
+ *   q, out, dout, dq  (batch, q_rows, heads, head_dim);  k, v, dk, dv  (batch, k_rows, kv_heads, head_dim)
+ *   heads % kv_heads == 0: query head h reads key head h / (heads / kv_heads);  head_dim % 8 == 0, 8 .. 512
+ *   stride_*[3]   elements between batches / rows / heads of q, k, v (and dout), multiples of 8 (0 = broadcast); the
+ *                 last dimension is contiguous, rows are 16-byte aligned.  out, dq, dk, dv are contiguous.
+ *   q_len, kv_len int32 DEVICE arrays (batch) or NULL = all rows; values are clamped to 0 .. q_rows / k_rows
+ *   causal        query i sees key j <= i + kv_len - q_len (the last query sees every key)
+ *   out[i] = sum_j softmax_j(scale q_i . k_j) v_j over the keys j < kv_len that i sees; lse[i] = log sum_j exp(scale q_i . k_j)
+ *            (batch, heads, q_rows) f32.  Rows i >= q_len and rows that see no key: out = 0, lse = -inf, no gradient.
+ *            Operand rows behind q_len / kv_len are never read; rows of dk / dv behind kv_len and of dq behind q_len are
+ *            written as zeros.  Keys and values in front of kv_len have to be finite also where `causal` hides them.
+ * Nothing is summed by atomics: equal calls give equal bits.  workspace: trace_attention_{fwd,bwd}_workspace_bytes(desc)
+ * bytes, 256-aligned (0: may be NULL); it is free again when the call's work on `stream` has ended. */
+typedef struct {
+  int batch, q_rows, k_rows, heads, kv_heads, head_dim;
+  int causal;
+  float scale; /* > 0 */
+  long long stride_q[3], stride_k[3], stride_v[3], stride_do[3];
+  const int32_t* q_len;
+  const int32_t* kv_len;
+} trace_attention_desc;
+size_t trace_attention_fwd_workspace_bytes(const trace_attention_desc* desc);
+int trace_attention_fwd_bf16(const trace_attention_desc* desc, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                             uint16_t* out, float* lse, void* workspace, size_t workspace_bytes, trace_stream_t stream);
+size_t trace_attention_bwd_workspace_bytes(const trace_attention_desc* desc);
+int trace_attention_bwd_bf16(const trace_attention_desc* desc, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                             const uint16_t* out, const float* lse, const uint16_t* dout, uint16_t* dq, uint16_t* dk,
+                             uint16_t* dv, void* workspace, size_t workspace_bytes, trace_stream_t stream);
+
+/* Group normalisation + activation over channels-last maps x (N, P, C), P = product of the positions, contiguous:
+ *   z = (x - mean) / sqrt(var + eps) * gamma + beta with the mean / biased variance of each sample's groups of C / G
+ *   channels, y = act(z); act = 0 | TRACE_EPI_RELU | TRACE_EPI_LEAKY | TRACE_EPI_SILU.  gamma / beta (C) f32, NULL = 1 / 0.
+ *   stats (N, G, 2) f32: mean and 1 / sqrt(var + eps), written by the forward call, read by the backward one.
+ *   backward: dx like x, dgamma / dbeta (C) f32 (each may be NULL).
+ * workspace: trace_group_norm_workspace_bytes(N, P, C, G, backward) bytes, 256-aligned.  Sums in f32 in a fixed order. */
+size_t trace_group_norm_workspace_bytes(int N, long long P, int C, int G, int backward);
+int trace_group_norm_act_bf16(const uint16_t* x, int N, long long P, int C, int G, const float* gamma, const float* beta,
+                              float eps, int act, uint16_t* y, float* stats, void* workspace, size_t workspace_bytes,
+                              trace_stream_t stream);
+int trace_group_norm_act_f32(const float* x, int N, long long P, int C, int G, const float* gamma, const float* beta,
+                             float eps, int act, float* y, float* stats, void* workspace, size_t workspace_bytes,
+                             trace_stream_t stream);
+int trace_group_norm_act_bwd_bf16(const uint16_t* x, const uint16_t* dy, int N, long long P, int C, int G,
+                                  const float* gamma, const float* beta, const float* stats, int act, uint16_t* dx,
+                                  float* dgamma, float* dbeta, void* workspace, size_t workspace_bytes,
+                                  trace_stream_t stream);
+int trace_group_norm_act_bwd_f32(const float* x, const float* dy, int N, long long P, int C, int G, const float* gamma,
+                                 const float* beta, const float* stats, int act, float* dx, float* dgamma, float* dbeta,
+                                 void* workspace, size_t workspace_bytes, trace_stream_t stream);
+
+/* Dropout + activation with a mask that is never stored (the Dropout -> LeakyReLU in front of the relation Linears,
+ * lib/modeling_rel/model_builder_rel.py:325-332): element i takes the (i % 8)-th 16-bit piece of
+ * Philox4x32-10(counter = (i / 8 as 64 bits, offset + *step as 64 bits), key = seed), low half of each word first, and is
+ * dropped where the piece < threshold (0 .. 65536);  y = act(x * 65536 / (65536 - threshold)) where kept, 0 where dropped
+ * (also for infinities and NaN).  act = 0 | TRACE_EPI_RELU | TRACE_EPI_LEAKY.  step: int64 DEVICE scalar or NULL = 0, so that
+ * the replays of a captured step draw other masks.  The backward call redraws the mask: dx = act'(x) dy * scale where kept;
+ * x may be NULL if act is 0.  y may be x, dx may be dy. */
+int trace_dropout_act_bf16(const uint16_t* x, long long n, int threshold, uint64_t seed, uint64_t offset, const int64_t* step,
+                           int act, uint16_t* y, trace_stream_t stream);
+int trace_dropout_act_f32(const float* x, long long n, int threshold, uint64_t seed, uint64_t offset, const int64_t* step,
+                          int act, float* y, trace_stream_t stream);
+int trace_dropout_act_bwd_bf16(const uint16_t* x, const uint16_t* dy, long long n, int threshold, uint64_t seed,
+                               uint64_t offset, const int64_t* step, int act, uint16_t* dx, trace_stream_t stream);
+int trace_dropout_act_bwd_f32(const float* x, const float* dy, long long n, int threshold, uint64_t seed, uint64_t offset,
+                              const int64_t* step, int act, float* dx, trace_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -24,7 +24,15 @@ class TreeGruWeights(ctypes.Structure):
                                         "Wzd", "Wrd", "Whd", "Uzd", "Urd", "Uhd", "bzd", "brd")]
 
 
+class AttentionDesc(ctypes.Structure):
+    _fields_ = ([(n, c_int) for n in ("batch", "q_rows", "k_rows", "heads", "kv_heads", "head_dim", "causal")]
+                + [("scale", c_float)]
+                + [(n, c_longlong * 3) for n in ("stride_q", "stride_k", "stride_v", "stride_do")]
+                + [("q_len", c_void_p), ("kv_len", c_void_p)])
+
+
 P = c_void_p
+c_u64 = ctypes.c_uint64
 # name -> (restype, argtypes); must list every symbol of include/trace_amd.h
 SIGNATURES = {
     "trace_last_error": (ctypes.c_char_p, []),
@@ -85,6 +93,19 @@ SIGNATURES = {
     "trace_tree_gru_ex": (c_int, [P, c_int, c_int, c_int, c_int, c_int, P, P, P, P, P, P,
                                   ctypes.POINTER(TreeGruWeights), c_int, P, P, P, c_size_t, P]),
     "trace_tree_gru_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "trace_attention_fwd_workspace_bytes": (c_size_t, [ctypes.POINTER(AttentionDesc)]),
+    "trace_attention_fwd_bf16": (c_int, [ctypes.POINTER(AttentionDesc), P, P, P, P, P, P, c_size_t, P]),
+    "trace_attention_bwd_workspace_bytes": (c_size_t, [ctypes.POINTER(AttentionDesc)]),
+    "trace_attention_bwd_bf16": (c_int, [ctypes.POINTER(AttentionDesc), P, P, P, P, P, P, P, P, P, P, c_size_t, P]),
+    "trace_group_norm_workspace_bytes": (c_size_t, [c_int, c_longlong, c_int, c_int, c_int]),
+    "trace_group_norm_act_bf16": (c_int, [P, c_int, c_longlong, c_int, c_int, P, P, c_float, c_int, P, P, P, c_size_t, P]),
+    "trace_group_norm_act_f32": (c_int, [P, c_int, c_longlong, c_int, c_int, P, P, c_float, c_int, P, P, P, c_size_t, P]),
+    "trace_group_norm_act_bwd_bf16": (c_int, [P, P, c_int, c_longlong, c_int, c_int, P, P, P, c_int, P, P, P, P, c_size_t, P]),
+    "trace_group_norm_act_bwd_f32": (c_int, [P, P, c_int, c_longlong, c_int, c_int, P, P, P, c_int, P, P, P, P, c_size_t, P]),
+    "trace_dropout_act_bf16": (c_int, [P, c_longlong, c_int, c_u64, c_u64, P, c_int, P, P]),
+    "trace_dropout_act_f32": (c_int, [P, c_longlong, c_int, c_u64, c_u64, P, c_int, P, P]),
+    "trace_dropout_act_bwd_bf16": (c_int, [P, P, c_longlong, c_int, c_u64, c_u64, P, c_int, P, P]),
+    "trace_dropout_act_bwd_f32": (c_int, [P, P, c_longlong, c_int, c_u64, c_u64, P, c_int, P, P]),
 }
 
 _lib = None

@@ -14,9 +14,13 @@ Operands are bf16 as in the forward pass (dy is rounded to bf16), accumulation f
 for the f32 master weights.  The strided views / zero stuffing / transposes around the kernels are torch indexing and
 `ops.transpose` - plumbing, not the product's arithmetic.  BatchNorm is handled by the caller (ConvModule.run_train):
 folded into the weights in eval mode, torch's batch_norm over the raw conv output in training mode.
+
+Softmax attention, group norm + activation and dropout + activation have kernels of their own for both directions
+(csrc/attention.hip, norm_ops.hip, dropout_ops.hip); their wrappers stand at the end.
 """
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -139,3 +143,73 @@ class _GemmNT(torch.autograd.Function):
 def gemm_nt(x, w, bias=None, relu=False):
     """Differentiable act(x @ w^T + bias): x (M,K) bf16, w (N,K) f32 (or bf16) master weights, K % 8 == 0."""
     return _GemmNT.apply(x, w, bias, bool(relu))
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, causal, q_len, kv_len):
+        out, lse = ops.attention(q, k, v, scale, causal, q_len, kv_len, return_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, q_len, kv_len)
+        ctx.cfg = (scale, causal)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        q, k, v, out, lse, q_len, kv_len = ctx.saved_tensors
+        grads = ops.attention_backward(gout.to(torch.bfloat16), q, k, v, out, lse, *ctx.cfg, q_len, kv_len)
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 4
+
+
+def attention(q, k, v, scale=None, causal=False, q_len=None, kv_len=None):
+    """Differentiable ops.attention (same arguments); gradients reach q, k and v.  Kept for the backward pass: the operands,
+    the output and one f32 per row - the probabilities are recomputed."""
+    return _Attention.apply(q, k, v, scale, bool(causal), q_len, kv_len)
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, groups, gamma, beta, eps, act):
+        y, stats = ops.group_norm_act(x, groups, gamma, beta, eps, act, return_stats=True)
+        ctx.save_for_backward(x, stats, gamma, beta)
+        ctx.cfg = (groups, act)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, stats, gamma, beta = ctx.saved_tensors
+        groups, act = ctx.cfg
+        need = ctx.needs_input_grad
+        dx, dg, db = ops.group_norm_act_backward(gy.to(x.dtype), x, stats, groups, gamma, beta, act, param_grads=need[2] or need[3])
+        return (dx if need[0] else None, None, dg.to(gamma.dtype) if need[2] else None, db.to(beta.dtype) if need[3] else None,
+                None, None)
+
+
+def group_norm_act(x, groups, gamma=None, beta=None, eps=1e-5, act=None):
+    """Differentiable ops.group_norm_act (same arguments); gradients reach x, gamma and beta.  Kept for the backward pass: x and
+    two f32 per (sample, group)."""
+    return _GroupNormAct.apply(x, int(groups), gamma, beta, float(eps), act)
+
+
+class _DropoutAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, offset, act, step):
+        y = ops.dropout_act(x, p, seed, offset, act, step)
+        ctx.save_for_backward(x if act not in (None, "none") else None, step)
+        ctx.cfg = (p, seed, offset, act, x.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, step = ctx.saved_tensors
+        p, seed, offset, act, dt = ctx.cfg
+        return (ops.dropout_act_backward(gy.to(dt), x, p, seed, offset, act, step),) + (None,) * 5
+
+
+def dropout_act(x, p, seed, offset=0, act=None, step=None, training=True):
+    """Differentiable ops.dropout_act (same arguments); without `training` nothing is dropped (p = 0).  Kept for the backward
+    pass: x where an activation follows, no mask.  `step` must not be advanced before the backward pass has been issued (autograd
+    reports it)."""
+    return _DropoutAct.apply(x, float(p) if training else 0.0, int(seed), int(offset), act, step)

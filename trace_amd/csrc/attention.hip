@@ -1,0 +1,882 @@
+// Softmax attention with its backward pass for gfx950: bf16 operands, f32 scores, statistics and sums.
+//
+//   forward    s = scale q k^T over the keys a query sees, out = softmax(s) v, lse = log sum exp(s)
+//   backward   P = exp(s - lse) (recomputed, never stored), delta_i = dout_i . out_i, dS = P (dout v^T - delta)
+//              dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout
+//
+// Layout that all three kernels share.  Every product runs on v_mfma_f32_16x16x32_bf16, whose result has its column in
+// the lane (lane & 15) and four consecutive rows 4 (lane >> 4) + r in the lane's registers.  The scores are formed with
+// the axis that the NEXT product sums over as rows: S^T (keys x queries) in the forward and dq kernels, S (queries x
+// keys) in the dk / dv kernel.  A lane then holds, for its own column, eight of the 32 summed rows of a pair of 16-row
+// tiles - rows {4 g + r} and {16 + 4 g + r}, g = lane >> 4 - and these, rounded to bf16, ARE the B operand of the next
+// product if its A operand lists the rows in the same order: no probability ever moves between lanes or through LDS.  The
+// A operand is the staged tile read transposed (ds_read_b64_tr_b16 on rows 4 g .. 4 g + 3 and 16 + 4 g ..), so one copy of
+// a tile in LDS serves both products it takes part in.  Softmax statistics belong to a column, so they live in the lane.
+//
+// Tiles of rows x head_dim go HBM / L2 -> LDS by 16-byte LDS-DMA, two stages deep; rows behind the sequence and columns
+// behind head_dim read a zero page, so nothing behind a length is ever touched.
+#include "lds_dma.h"
+#include <math.h>
+
+namespace trace {
+
+typedef __attribute__((ext_vector_type(8))) short at_s8;
+typedef __attribute__((ext_vector_type(4))) short at_s4;
+typedef __attribute__((ext_vector_type(4))) float at_f4;
+
+__device__ __attribute__((aligned(256))) const uint4 g_at_zero[16] = {};
+
+constexpr float AT_LOG2E = 1.4426950408889634f, AT_LN2 = 0.6931471805599453f;
+constexpr int AT_CUS = 256;
+
+struct AttnArgs {
+  const uint16_t *q, *k, *v, *out, *dout;
+  long long sq[3], sk[3], sv[3], sdo[3];   // elements between batches / rows / heads
+  int B, Nq, Nk, H, Hk, D, causal;
+  float scale;
+  const int32_t *q_len, *kv_len;
+  uint16_t *o, *dq, *dk, *dv;
+  float* lse;     // written by the forward, read by the backward kernels
+  float* delta;   // (B, H, Nq), backward
+  float* part;    // partial results of the splits (null: one split)
+  float2* part_ml;
+  int pack;       // query heads whose rows share one row axis (1, or all heads of a key head)
+  int units;      // heads / pack
+  int tiles, splits;
+};
+
+// LDS image of a tile: rows of 2 D bytes in 16-byte chunks, chunk c of row r at position c ^ at_key(r).  The key makes
+// both reads of a tile conflict-free over the 64 banks: a fragment read takes one chunk of 16 consecutive rows (16
+// different positions; 8 positions x 2 half-lines where a row is 128 bytes), a transposed read takes a 32-byte pair of
+// chunks of 8 consecutive rows (8 different pairs).
+template <int D> __device__ __forceinline__ int at_key(int r) {
+  return D >= 128 ? (((r & 7) << 1) | ((r >> 3) & 1)) : ((((r >> 1) & 3) << 1) | ((r >> 3) & 1));
+}
+template <int D> __device__ __forceinline__ int at_off(int r, int chunk) { return r * (2 * D) + ((chunk ^ at_key<D>(r)) << 4); }
+
+// One wave's share of the LDS-DMA of a ROWS x D tile (whole workgroup: NW waves).
+template <int D, int ROWS, int NW> struct AtLoader {
+  static constexpr int CPR = D / 8;
+  static constexpr int N = ROWS * CPR / (64 * NW);
+  static_assert(ROWS * CPR % (64 * NW) == 0, "whole instructions per wave");
+  const char* p[N];
+  unsigned colok;   // bit j: this lane's chunk of load j lies inside head_dim
+  long long step;   // bytes between rows
+  __device__ __forceinline__ void init(const uint16_t* base, long long row_stride, int d, int wave, int lane) {
+    colok = 0;
+    step = row_stride * 2;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int id = (j * NW + wave) * 64 + lane, row = id / CPR, c = (id % CPR) ^ at_key<D>(row);
+      p[j] = reinterpret_cast<const char*>(base) + row * step + c * 16;
+      if (c * 8 < d) colok |= 1u << j;
+    }
+  }
+  // rows row0 .. row0 + ROWS - 1 of the operand; rows >= row_end read zeros
+  __device__ __forceinline__ void issue(char* lds, int row0, int row_end, int wave, int lane) const {
+    const char* zero = reinterpret_cast<const char*>(g_at_zero);
+    const long long adv = row0 * step;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int row = ((j * NW + wave) * 64 + lane) / CPR;
+      const bool ok = ((colok >> j) & 1u) && row0 + row < row_end;
+      glds16(ok ? p[j] + adv : zero, lds + (j * NW + wave) * 1024);
+    }
+  }
+};
+
+// B operand: rows of a (rows x D) operand as columns of the product, read straight from memory (16 bytes per lane)
+template <int D> __device__ __forceinline__ void at_load_cols(at_s8 (&f)[D / 32], const uint16_t* row, bool ok, int d, int g) {
+#pragma unroll
+  for (int kc = 0; kc < D / 32; ++kc) {
+    const int c = kc * 32 + g * 8;
+    f[kc] = (ok && c < d) ? *reinterpret_cast<const at_s8*>(row + c) : at_s8{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+}
+
+__device__ __forceinline__ at_s8 at_pack8(const at_f4& a, const at_f4& b) {
+  union { at_s8 v; uint32_t u[4]; } o;
+  o.u[0] = pack_bf16x2(a[0], a[1]);
+  o.u[1] = pack_bf16x2(a[2], a[3]);
+  o.u[2] = pack_bf16x2(b[0], b[1]);
+  o.u[3] = pack_bf16x2(b[2], b[3]);
+  return o.v;
+}
+
+// A operand of the summing product: rows r0 + {4 g .. 4 g + 3} and r0 + 16 + {..} of the tile (k), columns 16 dt + (lane & 15) (m)
+template <int D> __device__ __forceinline__ at_s8 at_tr(const char* tile, int r0, int dt, int lane) {
+  const int g = lane >> 4, q = (lane >> 2) & 3, pq = lane & 3;
+  const int row = r0 + 4 * g + q, chunk = 2 * dt + (pq >> 1), half = (pq & 1) * 8;
+  const at_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_s4*)(tile + at_off<D>(row, chunk) + half));
+  const at_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_s4*)(tile + at_off<D>(row + 16, chunk) + half));
+  return at_s8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+}
+// A operand of a scoring product: rows r0 + (lane & 15), 8 columns from 32 kc + 8 g
+template <int D> __device__ __forceinline__ at_s8 at_row(const char* tile, int r0, int kc, int lane) {
+  return *reinterpret_cast<const at_s8*>(tile + at_off<D>(r0 + (lane & 15), kc * 4 + (lane >> 4)));
+}
+
+__device__ __forceinline__ at_f4 at_mfma(const at_s8& a, const at_s8& b, const at_f4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Workgroups go to the 8 XCDs round-robin and each XCD has its own L2: XCD x gets the x-th contiguous eighth of the
+// units, so the tiles that read one head's other operand share an L2.
+__device__ __forceinline__ int at_unit(int lin, int total) {
+  const int x = lin & 7, per = total >> 3, rem = total & 7;
+  return x * per + min(x, rem) + (lin >> 3);
+}
+__device__ __forceinline__ int at_len(const int32_t* len, int b, int n) { return len ? min(max(len[b], 0), n) : n; }
+
+__device__ __forceinline__ void at_store4(uint16_t* dst, float a, float b, float c, float d) {
+  uint2 o;
+  o.x = pack_bf16x2(a, b);
+  o.y = pack_bf16x2(c, d);
+  *reinterpret_cast<uint2*>(dst) = o;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Forward.  A workgroup owns NW * NT * 16 query rows of one (batch, head); with few query rows the rows of all heads that
+// share a key head form one row axis (`pack`), so the keys are read once for them.  Key tiles of BN rows; `splits`
+// workgroups share the keys of a row tile and leave (max, sum, unnormalised out) for attn_combine_kernel.
+// ---------------------------------------------------------------------------------------------------------------
+template <int D, int NT, int NW, int BN>
+__global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs p) {
+  constexpr int TR = NW * NT * 16, KC = D / 32, DT = D / 16, ST = BN / 16;
+  constexpr int TILE = BN * D * 2;
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of [K tile][V tile]
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int u = at_unit(blockIdx.x, gridDim.x);
+  int tile = u % p.tiles;
+  const int unit = (u / p.tiles) % p.units, b = u / p.tiles / p.units;
+  if (p.causal) tile = p.tiles - 1 - tile;   // the longest rows first
+  const int G = p.H / p.Hk, hk = unit * p.pack / G;
+  const int qlen = at_len(p.q_len, b, p.Nq), kvlen = at_len(p.kv_len, b, p.Nk), diff = kvlen - qlen;
+  const int nrows = p.pack * p.Nq;
+
+  int row_i[NT], row_h[NT], lim[NT];   // query, head and number of keys seen, of this lane's columns
+  at_s8 qf[NT][KC];
+  int wmin = 0x7fffffff, wmax = 0;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = tile * TR + (wave * NT + nt) * 16 + (lane & 15);
+    const int hh = p.pack > 1 ? r / p.Nq : 0;
+    row_h[nt] = unit * p.pack + hh;
+    row_i[nt] = r < nrows ? r - hh * p.Nq : -1;
+    const bool ok = row_i[nt] >= 0 && row_i[nt] < qlen;
+    lim[nt] = !ok ? 0 : p.causal ? min(max(row_i[nt] + diff + 1, 0), kvlen) : kvlen;
+    if (lim[nt] > 0) wmin = min(wmin, lim[nt]);
+    wmax = max(wmax, lim[nt]);
+    at_load_cols<D>(qf[nt], p.q + b * p.sq[0] + (ok ? row_i[nt] : 0) * p.sq[1] + (ok ? row_h[nt] : 0) * p.sq[2], ok, p.D, g);
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    wmin = min(wmin, __shfl_xor(wmin, o));
+    wmax = max(wmax, __shfl_xor(wmax, o));
+  }
+  wmin = __builtin_amdgcn_readfirstlane(wmin);
+  wmax = __builtin_amdgcn_readfirstlane(wmax);
+
+  int kend = 0;   // keys that some row of the workgroup sees
+  if (p.pack > 1) {
+    kend = qlen > 0 ? kvlen : 0;
+  } else {
+    const int last = min((tile + 1) * TR, qlen) - 1;
+    if (last >= tile * TR) kend = p.causal ? min(max(last + diff + 1, 0), kvlen) : kvlen;
+  }
+  const int ntile = (kend + BN - 1) / BN, per = (ntile + p.splits - 1) / p.splits;
+  const int t0 = min((int)blockIdx.y * per, ntile), t1 = min(t0 + per, ntile);
+
+  AtLoader<D, BN, NW> lk, lv;
+  lk.init(p.k + b * p.sk[0] + hk * p.sk[2], p.sk[1], p.D, wave, lane);
+  lv.init(p.v + b * p.sv[0] + hk * p.sv[2], p.sv[1], p.D, wave, lane);
+
+  const float c = p.scale * AT_LOG2E;
+  at_f4 acc[DT][NT];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt] = -INFINITY;
+    l[nt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (t0 < t1) {
+    lk.issue(smem, t0 * BN, kend, wave, lane);
+    lv.issue(smem + TILE, t0 * BN, kend, wave, lane);
+  }
+  for (int t = t0; t < t1; ++t) {
+    wait_vmcnt<0>();
+    ring_barrier();   // tile t landed for every wave; every wave is done reading the other stage
+    const char* kt = smem + ((t - t0) & 1) * (2 * TILE);
+    const char* vt = kt + TILE;
+    if (t + 1 < t1) {
+      char* nx = smem + ((t + 1 - t0) & 1) * (2 * TILE);
+      lk.issue(nx, (t + 1) * BN, kend, wave, lane);
+      lv.issue(nx + TILE, (t + 1) * BN, kend, wave, lane);
+    }
+    const int key0 = t * BN;
+    if (key0 >= wmax) continue;   // no row of this wave sees these keys
+    at_f4 s[ST][NT];
+#pragma unroll
+    for (int st = 0; st < ST; ++st) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[st][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc) {
+        const at_s8 a = at_row<D>(kt, st * 16, kc, lane);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[st][nt] = at_mfma(a, qf[nt][kc], s[st][nt]);
+      }
+    }
+    if (key0 + BN > wmin) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int st = 0; st < ST; ++st)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (key0 + st * 16 + 4 * g + r >= lim[nt]) s[st][nt][r] = -INFINITY;
+    }
+    at_s8 pf[BN / 32][NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float mx = m[nt];
+#pragma unroll
+      for (int st = 0; st < ST; ++st)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[st][nt][r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float base = mx == -INFINITY ? 0.f : mx * c;   // rows that saw nothing yet: exp2(-inf) = 0 below
+      const float alpha = __builtin_amdgcn_exp2f(m[nt] * c - base);
+      m[nt] = mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int st = 0; st < ST; ++st)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[st][nt][r] = __builtin_amdgcn_exp2f(s[st][nt][r] * c - base);
+          sum += s[st][nt][r];
+        }
+      l[nt] = l[nt] * alpha + sum;
+      if (__any(alpha != 1.f)) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt][nt] *= alpha;
+      }
+      // probabilities are rounded to bf16 for the product only (relative 2^-8 each, averaged over the row); their sum is not
+#pragma unroll
+      for (int kb = 0; kb < BN / 32; ++kb) pf[kb][nt] = at_pack8(s[2 * kb][nt], s[2 * kb + 1][nt]);
+    }
+#pragma unroll
+    for (int kb = 0; kb < BN / 32; ++kb)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const at_s8 a = at_tr<D>(vt, kb * 32, dt, lane);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, pf[kb][nt], acc[dt][nt]);
+      }
+  }
+  const bool split = p.splits > 1;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float sum = l[nt];
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (row_i[nt] < 0) continue;
+    const bool any = lim[nt] > 0 && sum > 0.f;
+    const long long row = ((long long)b * p.H + row_h[nt]) * p.Nq + row_i[nt];
+    if (split) {
+      const long long rows = (long long)p.B * p.H * p.Nq, at = blockIdx.y * rows + row;
+      if (g == 0) p.part_ml[at] = any ? make_float2(m[nt] * c, sum) : make_float2(-INFINITY, 0.f);
+      if (!any) continue;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        if (16 * dt + 4 * g < p.D) *reinterpret_cast<at_f4*>(p.part + at * p.D + 16 * dt + 4 * g) = acc[dt][nt];
+      continue;
+    }
+    if (g == 0 && p.lse) p.lse[row] = any ? (m[nt] * c + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
+    const float inv = any ? 1.f / sum : 0.f;
+    uint16_t* o = p.o + (((long long)b * p.Nq + row_i[nt]) * p.H + row_h[nt]) * p.D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int d = 16 * dt + 4 * g;
+      if (d < p.D) {
+        if (any) at_store4(o + d, acc[dt][nt][0] * inv, acc[dt][nt][1] * inv, acc[dt][nt][2] * inv, acc[dt][nt][3] * inv);
+        else at_store4(o + d, 0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  }
+}
+
+// out / lse of a row from its splits' (max, sum, unnormalised out), in split order; one thread per four columns
+__global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs p) {
+  const int dq = p.D >> 2;
+  const long long rows = (long long)p.B * p.H * p.Nq;
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= rows * dq) return;
+  const long long row = id / dq;
+  const int d = (int)(id - row * dq) * 4;
+  float mx = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, p.part_ml[s * rows + row].x);
+  float sum = 0.f;
+  at_f4 o = {0.f, 0.f, 0.f, 0.f};
+  if (mx != -INFINITY) {
+    for (int s = 0; s < p.splits; ++s) {
+      const float2 ml = p.part_ml[s * rows + row];
+      if (ml.y <= 0.f) continue;
+      const float w = __builtin_amdgcn_exp2f(ml.x - mx);
+      sum += w * ml.y;
+      o += w * *reinterpret_cast<const at_f4*>(p.part + (s * rows + row) * p.D + d);
+    }
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const int i = (int)(row % p.Nq), h = (int)(row / p.Nq % p.H);
+  const long long b = row / p.Nq / p.H;
+  at_store4(p.o + ((b * p.Nq + i) * p.H + h) * p.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  if (d == 0 && p.lse) p.lse[row] = sum > 0.f ? (mx + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// dq (and delta).  The same walk as the forward's over key tiles of 32, with two scoring products (q k^T and dout v^T).
+// ---------------------------------------------------------------------------------------------------------------
+template <int D, int NT, int NW>
+__global__ __launch_bounds__(64 * NW) void attn_bwd_q_kernel(const AttnArgs p) {
+  constexpr int BN = 32, TR = NW * NT * 16, KC = D / 32, DT = D / 16;
+  constexpr int TILE = BN * D * 2;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int u = at_unit(blockIdx.x, gridDim.x);
+  int tile = u % p.tiles;
+  const int h = (u / p.tiles) % p.H, b = u / p.tiles / p.H;
+  if (p.causal) tile = p.tiles - 1 - tile;
+  const int hk = h / (p.H / p.Hk);
+  const int qlen = at_len(p.q_len, b, p.Nq), kvlen = at_len(p.kv_len, b, p.Nk), diff = kvlen - qlen;
+
+  int row_i[NT], lim[NT];
+  float lse2[NT], delta[NT];
+  at_s8 qf[NT][KC], df[NT][KC];
+  int wmin = 0x7fffffff, wmax = 0;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int i = tile * TR + (wave * NT + nt) * 16 + (lane & 15);
+    row_i[nt] = i;
+    const bool ok = i < qlen;
+    lim[nt] = !ok ? 0 : p.causal ? min(max(i + diff + 1, 0), kvlen) : kvlen;
+    if (lim[nt] > 0) wmin = min(wmin, lim[nt]);
+    wmax = max(wmax, lim[nt]);
+    const int ii = ok ? i : 0;
+    at_load_cols<D>(qf[nt], p.q + b * p.sq[0] + ii * p.sq[1] + h * p.sq[2], ok, p.D, g);
+    at_load_cols<D>(df[nt], p.dout + b * p.sdo[0] + ii * p.sdo[1] + h * p.sdo[2], ok, p.D, g);
+    const uint16_t* orow = p.out + (((long long)b * p.Nq + ii) * p.H + h) * p.D;
+    float sum = 0.f;
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+      const int cc = kc * 32 + g * 8;
+      if (ok && cc < p.D) {
+        const at_s8 ov = *reinterpret_cast<const at_s8*>(orow + cc);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += bf16_to_f32((uint16_t)ov[e]) * bf16_to_f32((uint16_t)df[nt][kc][e]);
+      }
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    delta[nt] = sum;
+    const long long row = ((long long)b * p.H + h) * p.Nq + ii;
+    lse2[nt] = ok ? p.lse[row] * AT_LOG2E : 0.f;
+    if (ok && g == 0 && blockIdx.y == 0) p.delta[row] = sum;
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    wmin = min(wmin, __shfl_xor(wmin, o));
+    wmax = max(wmax, __shfl_xor(wmax, o));
+  }
+  wmin = __builtin_amdgcn_readfirstlane(wmin);
+  wmax = __builtin_amdgcn_readfirstlane(wmax);
+
+  int kend = 0;
+  const int last = min((tile + 1) * TR, qlen) - 1;
+  if (last >= tile * TR) kend = p.causal ? min(max(last + diff + 1, 0), kvlen) : kvlen;
+  const int ntile = (kend + BN - 1) / BN, per = (ntile + p.splits - 1) / p.splits;
+  const int t0 = min((int)blockIdx.y * per, ntile), t1 = min(t0 + per, ntile);
+
+  AtLoader<D, BN, NW> lk, lv;
+  lk.init(p.k + b * p.sk[0] + hk * p.sk[2], p.sk[1], p.D, wave, lane);
+  lv.init(p.v + b * p.sv[0] + hk * p.sv[2], p.sv[1], p.D, wave, lane);
+  const float c = p.scale * AT_LOG2E;
+  at_f4 acc[DT][NT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
+  if (t0 < t1) {
+    lk.issue(smem, t0 * BN, kend, wave, lane);
+    lv.issue(smem + TILE, t0 * BN, kend, wave, lane);
+  }
+  for (int t = t0; t < t1; ++t) {
+    wait_vmcnt<0>();
+    ring_barrier();
+    const char* kt = smem + ((t - t0) & 1) * (2 * TILE);
+    const char* vt = kt + TILE;
+    if (t + 1 < t1) {
+      char* nx = smem + ((t + 1 - t0) & 1) * (2 * TILE);
+      lk.issue(nx, (t + 1) * BN, kend, wave, lane);
+      lv.issue(nx + TILE, (t + 1) * BN, kend, wave, lane);
+    }
+    const int key0 = t * BN;
+    if (key0 >= wmax) continue;
+    at_f4 s[2][NT], dp[2][NT];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[st][nt] = dp[st][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc) {
+        const at_s8 a = at_row<D>(kt, st * 16, kc, lane), av = at_row<D>(vt, st * 16, kc, lane);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          s[st][nt] = at_mfma(a, qf[nt][kc], s[st][nt]);
+          dp[st][nt] = at_mfma(av, df[nt][kc], dp[st][nt]);
+        }
+      }
+    }
+    const bool mask = key0 + BN > wmin;
+    at_s8 ds[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float pr = __builtin_amdgcn_exp2f(s[st][nt][r] * c - lse2[nt]);
+          if (mask && key0 + st * 16 + 4 * g + r >= lim[nt]) pr = 0.f;
+          s[st][nt][r] = pr * (dp[st][nt][r] - delta[nt]);
+        }
+      ds[nt] = at_pack8(s[0][nt], s[1][nt]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const at_s8 a = at_tr<D>(kt, 0, dt, lane);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, ds[nt], acc[dt][nt]);
+    }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    if (row_i[nt] >= p.Nq) continue;
+    const bool any = lim[nt] > 0;
+    const long long at = (((long long)b * p.Nq + row_i[nt]) * p.H + h) * p.D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int d = 16 * dt + 4 * g;
+      if (d >= p.D) continue;
+      const at_f4 a = any ? acc[dt][nt] : at_f4{0.f, 0.f, 0.f, 0.f};
+      if (p.splits > 1)
+        *reinterpret_cast<at_f4*>(p.part + blockIdx.y * ((long long)p.B * p.Nq * p.H * p.D) + at + d) = a;
+      else
+        at_store4(p.dq + at + d, a[0] * p.scale, a[1] * p.scale, a[2] * p.scale, a[3] * p.scale);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// dk and dv.  A workgroup owns NW * NT * 16 keys of one (batch, key head) - in registers as B operands - and walks the
+// 32-row tiles of q and dout of every query head that reads it, so the gradients of shared heads are summed in a fixed order.
+// ---------------------------------------------------------------------------------------------------------------
+template <int D, int NT, int NW>
+__global__ __launch_bounds__(64 * NW) void attn_bwd_kv_kernel(const AttnArgs p) {
+  constexpr int BQ = 32, TK = NW * NT * 16, KC = D / 32, DT = D / 16;
+  constexpr int TILE = BQ * D * 2, STAGE = 2 * TILE + 256;   // [q][dout][32 lse, 32 delta]
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int u = at_unit(blockIdx.x, gridDim.x);
+  const int tile = u % p.tiles, hk = (u / p.tiles) % p.Hk, b = u / p.tiles / p.Hk;
+  const int G = p.H / p.Hk;
+  const int qlen = at_len(p.q_len, b, p.Nq), kvlen = at_len(p.kv_len, b, p.Nk), diff = kvlen - qlen;
+  const int key_first = tile * TK, wkey = key_first + wave * NT * 16;
+
+  int key[NT];
+  at_s8 kf[NT][KC], vf[NT][KC];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    key[nt] = wkey + nt * 16 + (lane & 15);
+    const bool ok = key[nt] < kvlen;
+    const int kk = ok ? key[nt] : 0;
+    at_load_cols<D>(kf[nt], p.k + b * p.sk[0] + kk * p.sk[1] + hk * p.sk[2], ok, p.D, g);
+    at_load_cols<D>(vf[nt], p.v + b * p.sv[0] + kk * p.sv[1] + hk * p.sv[2], ok, p.D, g);
+  }
+  at_f4 ak[DT][NT], av[DT][NT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) ak[dt][nt] = av[dt][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
+
+  // query tiles qt0 .. nq - 1 of each of the G heads, as one list of which this split takes a part
+  const int nq = key_first < kvlen ? (qlen + BQ - 1) / BQ : 0;
+  const int qt0 = p.causal ? min(max(key_first - diff, 0) / BQ, nq) : 0;
+  const int per_head = nq - qt0, n_it = per_head * G, per = (n_it + p.splits - 1) / p.splits;
+  const int it0 = min((int)blockIdx.y * per, n_it), it1 = min(it0 + per, n_it);
+
+  AtLoader<D, BQ, NW> lq, ld;
+  lq.init(p.q + b * p.sq[0] + (long long)hk * G * p.sq[2], p.sq[1], p.D, wave, lane);
+  ld.init(p.dout + b * p.sdo[0] + (long long)hk * G * p.sdo[2], p.sdo[1], p.D, wave, lane);
+  const long long head_q = p.sq[2] * 2, head_do = p.sdo[2] * 2;
+  const float* stat = (lane < 32 ? p.lse : p.delta) + ((long long)b * p.H + (long long)hk * G) * p.Nq;
+
+  auto issue = [&](char* st, int it) {
+    const int hh = it / per_head, q0 = (qt0 + it - hh * per_head) * BQ;
+    AtLoader<D, BQ, NW> a = lq, d = ld;
+#pragma unroll
+    for (int j = 0; j < AtLoader<D, BQ, NW>::N; ++j) {
+      a.p[j] += hh * head_q;
+      d.p[j] += hh * head_do;
+    }
+    a.issue(st, q0, qlen, wave, lane);
+    d.issue(st + TILE, q0, qlen, wave, lane);
+    if (wave == 0) {
+      const int i = q0 + (lane & 31);
+      const float* src = i < qlen ? stat + (long long)hh * p.Nq + i : reinterpret_cast<const float*>(g_at_zero);
+      __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(st + 2 * TILE), 4, 0, 0);
+    }
+  };
+  const float c = p.scale * AT_LOG2E;
+  if (it0 < it1) issue(smem, it0);
+  for (int it = it0; it < it1; ++it) {
+    wait_vmcnt<0>();
+    ring_barrier();
+    const char* qt = smem + ((it - it0) & 1) * STAGE;
+    const char* dt_ = qt + TILE;
+    const float* st_ = reinterpret_cast<const float*>(qt + 2 * TILE);
+    if (it + 1 < it1) issue(smem + ((it + 1 - it0) & 1) * STAGE, it + 1);
+    const int q0 = (qt0 + it % per_head) * BQ;
+    if (p.causal && wkey > q0 + BQ - 1 + diff) continue;   // no key of this wave is seen
+    at_f4 s[2][NT], dp[2][NT];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[st][nt] = dp[st][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc) {
+        const at_s8 a = at_row<D>(qt, st * 16, kc, lane), ad = at_row<D>(dt_, st * 16, kc, lane);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          s[st][nt] = at_mfma(a, kf[nt][kc], s[st][nt]);
+          dp[st][nt] = at_mfma(ad, vf[nt][kc], dp[st][nt]);
+        }
+      }
+    }
+    const bool mask = q0 + BQ > qlen || wkey + NT * 16 > kvlen || (p.causal && wkey + NT * 16 - 1 > q0 + diff);
+    at_s8 pf[NT], ds[NT];
+    at_f4 lse2[2], del[2];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      lse2[st] = *reinterpret_cast<const at_f4*>(st_ + st * 16 + 4 * g) * AT_LOG2E;
+      del[st] = *reinterpret_cast<const at_f4*>(st_ + 32 + st * 16 + 4 * g);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float pr = __builtin_amdgcn_exp2f(s[st][nt][r] * c - lse2[st][r]);
+          const int i = q0 + st * 16 + 4 * g + r;
+          if (mask && (i >= qlen || key[nt] >= kvlen || (p.causal && key[nt] > i + diff))) pr = 0.f;
+          s[st][nt][r] = pr;
+          dp[st][nt][r] = pr * (dp[st][nt][r] - del[st][r]);
+        }
+      pf[nt] = at_pack8(s[0][nt], s[1][nt]);
+      ds[nt] = at_pack8(dp[0][nt], dp[1][nt]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const at_s8 a = at_tr<D>(dt_, 0, dt, lane), aq = at_tr<D>(qt, 0, dt, lane);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        av[dt][nt] = at_mfma(a, pf[nt], av[dt][nt]);
+        ak[dt][nt] = at_mfma(aq, ds[nt], ak[dt][nt]);
+      }
+    }
+  }
+  const long long n_all = (long long)p.B * p.Nk * p.Hk * p.D;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    if (key[nt] >= p.Nk) continue;
+    const long long at = (((long long)b * p.Nk + key[nt]) * p.Hk + hk) * p.D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int d = 16 * dt + 4 * g;
+      if (d >= p.D) continue;
+      const at_f4 a = ak[dt][nt], w = av[dt][nt];
+      if (p.splits > 1) {
+        float* dst = p.part + (long long)blockIdx.y * 2 * n_all + at + d;
+        *reinterpret_cast<at_f4*>(dst) = a;
+        *reinterpret_cast<at_f4*>(dst + n_all) = w;
+      } else {
+        at_store4(p.dk + at + d, a[0] * p.scale, a[1] * p.scale, a[2] * p.scale, a[3] * p.scale);
+        at_store4(p.dv + at + d, w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+}
+
+// dst = bf16(mul * sum over splits), in split order; four elements per thread, n % 8 == 0
+__global__ __launch_bounds__(256) void attn_reduce_kernel(const float* __restrict__ part, long long split_stride, int splits,
+                                                          long long n, float mul, uint16_t* __restrict__ dst) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  at_f4 a = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) a += *reinterpret_cast<const at_f4*>(part + s * split_stride + i);
+  at_store4(dst + i, a[0] * mul, a[1] * mul, a[2] * mul, a[3] * mul);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Host: one rule for a call's tiles and splits, used for the workspace size and for the launch.
+// ---------------------------------------------------------------------------------------------------------------
+struct AttnPlan {
+  int D;                                   // head_dim rounded up to a built size
+  int pack, units, tile_rows, tiles, splits;   // forward
+  int q_rows, q_tiles, q_splits;           // dq
+  int k_rows, k_tiles, k_splits;           // dk / dv
+};
+
+static inline size_t at_align(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Splits so that about two workgroups per CU exist, each with at least `min_iters` iterations of its loop.
+static int at_splits(long long groups, int iters, int min_iters) {
+  if (groups >= AT_CUS || groups <= 0) return 1;
+  long long s = (2 * AT_CUS + groups - 1) / groups;
+  const long long most = iters / min_iters;
+  if (s > most) s = most;
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : (int)s;
+}
+
+static AttnPlan at_plan(const trace_attention_desc* d) {
+  AttnPlan pl;
+  const int hd = d->head_dim;
+  pl.D = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
+  const int G = d->heads / d->kv_heads;
+  // few query rows: all heads of a key head on one row axis, 16 rows per workgroup (its one wave streams the keys)
+  const bool small = (long long)d->q_rows * G <= 16;
+  pl.pack = small ? G : 1;
+  pl.units = d->heads / pl.pack;
+  pl.tile_rows = small ? 16 : pl.D <= 256 ? 128 : 64;
+  pl.tiles = ceil_div((long long)pl.pack * d->q_rows, pl.tile_rows);
+  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch * (small ? 1 : 1), ceil_div(d->k_rows, 32), 4);
+  const int bwd_rows = pl.D == 64 ? 256 : pl.D == 128 ? 128 : pl.D == 256 ? 64 : 64;
+  pl.q_rows = bwd_rows;
+  pl.q_tiles = ceil_div(d->q_rows, pl.q_rows);
+  pl.q_splits = at_splits((long long)pl.q_tiles * d->heads * d->batch, ceil_div(d->k_rows, 32), 4);
+  pl.k_rows = bwd_rows;
+  pl.k_tiles = ceil_div(d->k_rows, pl.k_rows);
+  pl.k_splits = at_splits((long long)pl.k_tiles * d->kv_heads * d->batch, ceil_div(d->q_rows, 32) * G, 4);
+  return pl;
+}
+
+static int at_check(const trace_attention_desc* d, const char* what) {
+  TRACE_REQUIRE(d, "%s: null descriptor", what);
+  TRACE_REQUIRE(d->batch >= 0 && d->q_rows >= 0 && d->k_rows >= 0 && d->heads > 0 && d->kv_heads > 0, "%s: bad sizes", what);
+  TRACE_REQUIRE(d->heads % d->kv_heads == 0, "%s: heads (%d) must be a multiple of kv_heads (%d)", what, d->heads, d->kv_heads);
+  TRACE_REQUIRE(d->head_dim >= 8 && d->head_dim <= 512 && d->head_dim % 8 == 0, "%s: head_dim %d (8 .. 512, multiple of 8)",
+                what, d->head_dim);
+  TRACE_REQUIRE(d->scale > 0.f && d->scale <= 3.0e38f, "%s: scale must be positive and finite", what);
+  // tiles x heads x batch are grid indices and rows x heads of a packed call row indices
+  TRACE_REQUIRE((long long)d->batch * d->heads * ((long long)d->q_rows + d->k_rows + 2) < (1ll << 31) - 1, "%s: too many rows", what);
+  for (int i = 0; i < 3; ++i)
+    TRACE_REQUIRE(((d->stride_q[i] | d->stride_k[i] | d->stride_v[i]) & 7) == 0, "%s: strides must be multiples of 8 elements", what);
+  return 0;
+}
+
+static AttnArgs at_args(const trace_attention_desc* d, const uint16_t* q, const uint16_t* k, const uint16_t* v) {
+  AttnArgs a = {};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  for (int i = 0; i < 3; ++i) {
+    a.sq[i] = d->stride_q[i];
+    a.sk[i] = d->stride_k[i];
+    a.sv[i] = d->stride_v[i];
+    a.sdo[i] = d->stride_do[i];
+  }
+  a.B = d->batch;
+  a.Nq = d->q_rows;
+  a.Nk = d->k_rows;
+  a.H = d->heads;
+  a.Hk = d->kv_heads;
+  a.D = d->head_dim;
+  a.causal = d->causal ? 1 : 0;
+  a.scale = d->scale;
+  a.q_len = d->q_len;
+  a.kv_len = d->kv_len;
+  return a;
+}
+
+static bool at_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <int D, int NT, int NW, int BN> static int at_launch_fwd(const AttnArgs& a, hipStream_t st) {
+  const int lds = 2 * 2 * BN * D * 2;
+  TRACE_LDS_OPT_IN((attn_fwd_kernel<D, NT, NW, BN>), lds, "attention");
+  attn_fwd_kernel<D, NT, NW, BN><<<dim3((unsigned)a.tiles * a.units * a.B, a.splits), 64 * NW, lds, st>>>(a);
+  return 0;
+}
+template <int D, int NT, int NW> static int at_launch_q(const AttnArgs& a, hipStream_t st) {
+  const int lds = 2 * 2 * 32 * D * 2;
+  TRACE_LDS_OPT_IN((attn_bwd_q_kernel<D, NT, NW>), lds, "attention backward");
+  attn_bwd_q_kernel<D, NT, NW><<<dim3((unsigned)a.tiles * a.H * a.B, a.splits), 64 * NW, lds, st>>>(a);
+  return 0;
+}
+template <int D, int NT, int NW> static int at_launch_kv(const AttnArgs& a, hipStream_t st) {
+  const int lds = 2 * (2 * 32 * D * 2 + 256);
+  TRACE_LDS_OPT_IN((attn_bwd_kv_kernel<D, NT, NW>), lds, "attention backward");
+  attn_bwd_kv_kernel<D, NT, NW><<<dim3((unsigned)a.tiles * a.Hk * a.B, a.splits), 64 * NW, lds, st>>>(a);
+  return 0;
+}
+
+}  // namespace trace
+
+using namespace trace;
+
+static size_t at_fwd_bytes(const trace_attention_desc* d, const AttnPlan& pl) {
+  if (pl.splits <= 1) return 0;
+  const size_t rows = (size_t)d->batch * d->heads * d->q_rows;
+  return at_align(pl.splits * rows * sizeof(float2)) + at_align(pl.splits * rows * d->head_dim * sizeof(float));
+}
+
+extern "C" size_t trace_attention_fwd_workspace_bytes(const trace_attention_desc* d) {
+  if (at_check(d, "attention")) return 0;
+  return at_fwd_bytes(d, at_plan(d));
+}
+
+extern "C" int trace_attention_fwd_bf16(const trace_attention_desc* d, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                                        uint16_t* out, float* lse, void* workspace, size_t workspace_bytes,
+                                        trace_stream_t stream) {
+  if (int rc = at_check(d, "attention")) return rc;
+  if (d->batch == 0 || d->q_rows == 0) return 0;
+  TRACE_REQUIRE(q && out && (d->k_rows == 0 || (k && v)), "attention: null pointer");
+  TRACE_REQUIRE(at_aligned(q) && at_aligned(k) && at_aligned(v) && at_aligned(out), "attention: operands must be 16-byte aligned");
+  const AttnPlan pl = at_plan(d);
+  const size_t need = at_fwd_bytes(d, pl);
+  TRACE_REQUIRE(workspace_bytes >= need && (!need || workspace), "attention: workspace of %zu bytes needed", need);
+  AttnArgs a = at_args(d, q, k, v);
+  a.o = out;
+  a.lse = lse;
+  a.pack = pl.pack;
+  a.units = pl.units;
+  a.tiles = pl.tiles;
+  a.splits = pl.splits;
+  const long long rows = (long long)d->batch * d->heads * d->q_rows;
+  if (pl.splits > 1) {
+    a.part_ml = reinterpret_cast<float2*>(workspace);
+    a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + at_align(pl.splits * rows * sizeof(float2)));
+  }
+  hipStream_t st = (hipStream_t)stream;
+  int rc = 0;
+  if (pl.tile_rows == 16) {
+    switch (pl.D) {
+      case 64: rc = at_launch_fwd<64, 1, 1, 32>(a, st); break;
+      case 128: rc = at_launch_fwd<128, 1, 1, 32>(a, st); break;
+      case 256: rc = at_launch_fwd<256, 1, 1, 32>(a, st); break;
+      default: rc = at_launch_fwd<512, 1, 1, 32>(a, st); break;
+    }
+  } else {
+    switch (pl.D) {
+      case 64: rc = at_launch_fwd<64, 2, 4, 64>(a, st); break;
+      case 128: rc = at_launch_fwd<128, 2, 4, 64>(a, st); break;
+      case 256: rc = at_launch_fwd<256, 2, 4, 32>(a, st); break;
+      default: rc = at_launch_fwd<512, 1, 4, 32>(a, st); break;
+    }
+  }
+  if (rc) return rc;
+  if (int e = check_launch("attention")) return e;
+  if (pl.splits > 1) {
+    attn_combine_kernel<<<ceil_div(rows * (d->head_dim / 4), 256), 256, 0, st>>>(a);
+    return check_launch("attention combine");
+  }
+  return 0;
+}
+
+struct AttnBwdBytes {
+  size_t delta, q, kv;
+};
+static AttnBwdBytes at_bwd_bytes(const trace_attention_desc* d, const AttnPlan& pl) {
+  AttnBwdBytes s;
+  s.delta = at_align((size_t)d->batch * d->heads * d->q_rows * sizeof(float));
+  s.q = pl.q_splits > 1 ? at_align((size_t)pl.q_splits * d->batch * d->q_rows * d->heads * d->head_dim * sizeof(float)) : 0;
+  s.kv = pl.k_splits > 1 ? at_align((size_t)pl.k_splits * 2 * d->batch * d->k_rows * d->kv_heads * d->head_dim * sizeof(float)) : 0;
+  return s;
+}
+
+extern "C" size_t trace_attention_bwd_workspace_bytes(const trace_attention_desc* d) {
+  if (at_check(d, "attention backward")) return 0;
+  const AttnBwdBytes s = at_bwd_bytes(d, at_plan(d));
+  return s.delta + (s.q > s.kv ? s.q : s.kv);   // the splits of dq are reduced before those of dk / dv are written
+}
+
+extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                                        const uint16_t* out, const float* lse, const uint16_t* dout, uint16_t* dq, uint16_t* dk,
+                                        uint16_t* dv, void* workspace, size_t workspace_bytes, trace_stream_t stream) {
+  if (int rc = at_check(d, "attention backward")) return rc;
+  for (int i = 0; i < 3; ++i)
+    TRACE_REQUIRE((d->stride_do[i] & 7) == 0, "attention backward: strides must be multiples of 8 elements");
+  if (d->batch == 0) return 0;
+  TRACE_REQUIRE(d->q_rows == 0 || (q && out && lse && dout && dq), "attention backward: null pointer");
+  TRACE_REQUIRE(d->k_rows == 0 || (k && v && dk && dv), "attention backward: null pointer");
+  TRACE_REQUIRE(at_aligned(q) && at_aligned(k) && at_aligned(v) && at_aligned(out) && at_aligned(dout) && at_aligned(dq) &&
+                    at_aligned(dk) && at_aligned(dv),
+                "attention backward: operands must be 16-byte aligned");
+  const AttnPlan pl = at_plan(d);
+  const AttnBwdBytes s = at_bwd_bytes(d, pl);
+  const size_t need = s.delta + (s.q > s.kv ? s.q : s.kv);
+  TRACE_REQUIRE(workspace_bytes >= need && (!need || workspace), "attention backward: workspace of %zu bytes needed", need);
+  AttnArgs a = at_args(d, q, k, v);
+  a.out = out;
+  a.dout = dout;
+  a.lse = const_cast<float*>(lse);
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.delta = reinterpret_cast<float*>(workspace);
+  a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + s.delta);
+  hipStream_t st = (hipStream_t)stream;
+  int rc = 0;
+  if (d->q_rows > 0) {
+    a.tiles = pl.q_tiles;
+    a.splits = pl.q_splits;
+    switch (pl.D) {
+      case 64: rc = at_launch_q<64, 4, 4>(a, st); break;
+      case 128: rc = at_launch_q<128, 2, 4>(a, st); break;
+      case 256: rc = at_launch_q<256, 1, 4>(a, st); break;
+      default: rc = at_launch_q<512, 1, 4>(a, st); break;
+    }
+    if (rc) return rc;
+    if (int e = check_launch("attention backward (dq)")) return e;
+    if (pl.q_splits > 1) {
+      const long long n = (long long)d->batch * d->q_rows * d->heads * d->head_dim;
+      attn_reduce_kernel<<<ceil_div(n, 1024), 256, 0, st>>>(a.part, n, pl.q_splits, n, d->scale, dq);
+      if (int e = check_launch("attention backward (dq splits)")) return e;
+    }
+  }
+  if (d->k_rows > 0) {
+    a.tiles = pl.k_tiles;
+    a.splits = pl.k_splits;
+    switch (pl.D) {
+      case 64: rc = at_launch_kv<64, 4, 4>(a, st); break;
+      case 128: rc = at_launch_kv<128, 2, 4>(a, st); break;
+      case 256: rc = at_launch_kv<256, 1, 4>(a, st); break;
+      default: rc = at_launch_kv<512, 1, 4>(a, st); break;
+    }
+    if (rc) return rc;
+    if (int e = check_launch("attention backward (dk, dv)")) return e;
+    if (pl.k_splits > 1) {
+      const long long n = (long long)d->batch * d->k_rows * d->kv_heads * d->head_dim;
+      attn_reduce_kernel<<<ceil_div(n, 1024), 256, 0, st>>>(a.part, 2 * n, pl.k_splits, n, d->scale, dk);
+      attn_reduce_kernel<<<ceil_div(n, 1024), 256, 0, st>>>(a.part + n, 2 * n, pl.k_splits, n, 1.0f, dv);
+      if (int e = check_launch("attention backward (dk, dv splits)")) return e;
+    }
+  }
+  return 0;
+}

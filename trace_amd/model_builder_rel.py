@@ -1267,6 +1267,23 @@ class Generalized_RCNN(PackedLinears):
         return dict(det_labels=det_labels, det_scores=det_scores, sbj_labels=sbj_lab_all, obj_labels=obj_lab_all,
                     sbj_scores=sbj_sc_all, obj_scores=obj_sc_all, msp_det_scores=obj_score, prd_scores=prd, top=top)
 
+    def relation_logits_train(self, sem, spatio, seed, offset=0, so_part=None, step=None):
+        """The two relation MLPs under autograd (lib/modeling_rel/model_builder_rel.py:325-332, 1066-1069): logits =
+        relation_infer_sem(sem) + relation_infer_spa(spatio) (+ so_part), each Dropout -> LeakyReLU(0.1) -> Linear, as
+        dropout_act + gemm_nt.  sem / spatio (P, infer) bf16 or f32 features in front of the Dropout -> (P, NUM_PRD_CLASSES)
+        f32.  In training mode the masks are functions of (seed, offset + step) - sem draws from `seed`, spatio from
+        `seed` ^ 1 -, so a caller advances `offset` (or the device scalar `step`, for a captured step) every step; in eval
+        mode nothing is dropped."""
+        from . import autograd as tag
+        total = None if so_part is None else so_part.float()
+        for x, seq, key in ((sem, self.relation_infer_sem, int(seed)), (spatio, self.relation_infer_spa, int(seed) ^ 1)):
+            h = tag.dropout_act(x, seq[0].p, key, offset, "leaky", step, training=self.training)
+            w, b = seq[2].weight, seq[2].bias
+            pad = -w.shape[0] % 8
+            y = tag.gemm_nt(h, F.pad(w, (0, 0, 0, pad)), F.pad(b, (0, pad)))[:, :w.shape[0]].float()
+            total = y if total is None else total + y
+        return total
+
     @staticmethod
     def _make_outs(prep, res, topk, prd_k):
         """Per-clip return dicts (:1162-1182): views into the step's flat tensors + the host-side roi lists."""

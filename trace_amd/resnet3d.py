@@ -29,33 +29,40 @@ _PACK_EPOCH = [0]
 
 class ConvModule(nn.Module):
     """mmcv.cnn.ConvModule subset used by resnet3d.py: conv -> bn -> ReLU.
-    bias='auto' means "bias iff no norm" (mmcv semantics)."""
+    bias='auto' means "bias iff no norm" (mmcv semantics).  norm_cfg=dict(type='GN', num_groups=..) (mmcv's name for it; eps and
+    requires_grad as there) takes nn.GroupNorm as `gn` instead of the BatchNorm `bn`: its statistics belong to one clip, so it
+    trains at any batch size, but it cannot be folded into the weights."""
 
     def __init__(self, in_channels, out_channels, kernel_size, stride=1, padding=0, dilation=1, bias='auto',
                  conv_cfg=None, norm_cfg=None, act_cfg=dict(type='ReLU')):
         super().__init__()
         self.with_norm = norm_cfg is not None
+        self.with_gn = self.with_norm and norm_cfg.get('type') == 'GN'
         self.with_activation = act_cfg is not None
         if bias == 'auto':
             bias = not self.with_norm
         self.conv = nn.Conv3d(in_channels, out_channels, _triple(kernel_size), _triple(stride), _triple(padding),
                               _triple(dilation), bias=bias)
-        if self.with_norm:
+        if self.with_gn:
+            self.gn = nn.GroupNorm(norm_cfg['num_groups'], out_channels, eps=norm_cfg.get('eps', 1e-5))
+            for t in self.gn.parameters():
+                t.requires_grad_(norm_cfg.get('requires_grad', True))
+        elif self.with_norm:
             self.bn = nn.BatchNorm3d(out_channels)
         self._packed = None
 
     @property
     def norm(self):
-        return self.bn if self.with_norm else None
+        return self.gn if self.with_gn else self.bn if self.with_norm else None
 
     def packed(self):
-        """(w (Cout, taps*Cin) bf16 with BN scale folded, bias (Cout) f32)."""
+        """(w (Cout, taps*Cin) bf16 with BN scale folded, bias (Cout) f32); of the bare convolution with a GroupNorm."""
         if self._packed is not None and self._packed[2] != _PACK_EPOCH[0]:
             self._packed = None       # BN buffers / weights were reloaded somewhere in the tree since this was folded
         if self._packed is None:
             w = self.conv.weight.detach().float()
             cout = w.shape[0]
-            if self.with_norm:
+            if self.with_norm and not self.with_gn:
                 scale = self.bn.weight.detach().float() / torch.sqrt(self.bn.running_var.float() + self.bn.eps)
                 shift = self.bn.bias.detach().float() - self.bn.running_mean.float() * scale
             else:
@@ -73,7 +80,7 @@ class ConvModule(nn.Module):
         calibrating synthetic BN statistics; the inference hot path is `run`."""
         x = self.conv(x)
         if self.with_norm:
-            x = self.bn(x)
+            x = self.norm(x)
         return torch.relu(x) if self.with_activation else x
 
     def run(self, x, residual=None, relu=None, pool_t2=False):
@@ -81,17 +88,36 @@ class ConvModule(nn.Module):
         w, b = self.packed()
         c = self.conv
         relu = self.with_activation if relu is None else relu
+        if self.with_gn:
+            y = ops.conv3d(x, w, b, c.kernel_size, c.stride, c.padding, c.dilation)
+            y = self._group_norm(y, relu and residual is None)
+            if residual is not None:
+                y = y + residual
+                y = torch.relu_(y) if relu else y
+            return ops.maxpool3d(y, (2, 1, 1), (2, 1, 1)) if pool_t2 else y
         return ops.conv3d(x, w, b, c.kernel_size, c.stride, c.padding, c.dilation, residual=residual, relu=relu,
                           pool_t2=pool_t2)
+
+    def _group_norm(self, y, relu):
+        gn = self.gn
+        return ops.group_norm_act(y, gn.num_groups, gn.weight.detach().float(), gn.bias.detach().float(), gn.eps,
+                                  "relu" if relu else None)
 
     def run_train(self, x, relu=None):
         """`run` under autograd (trace_amd/autograd.py); the convolution and both of its gradients run on the HIP kernels.
         BatchNorm in eval mode (norm_eval, frozen stages): the fold is taken differentiably from the f32 parameters
         (running_mean / running_var are constants).  BatchNorm in training mode: batch statistics, see below.
-        Gradients reach conv.weight, conv.bias, bn.weight, bn.bias and x."""
+        GroupNorm: the raw convolution, then the normalisation with its activation as one operator (ops.group_norm_act).
+        Gradients reach conv.weight, conv.bias, the norm's weight and bias and x."""
         from . import autograd as tag
         w = self.conv.weight.float()
         cout = w.shape[0]
+        if self.with_gn:
+            c, gn = self.conv, self.gn
+            y = tag.conv3d(x, w.permute(0, 2, 3, 4, 1).reshape(cout, -1), None if c.bias is None else c.bias.float(),
+                           c.kernel_size, c.stride, c.padding, c.dilation, relu=False)
+            relu = self.with_activation if relu is None else relu
+            return tag.group_norm_act(y, gn.num_groups, gn.weight, gn.bias, gn.eps, "relu" if relu else None)
         if self.with_norm and self.bn.training:
             # batch statistics (the reference's I3D config trains with norm_eval=False: lib/i3d/resnet3d.py:804-811 leaves
             # the BatchNorm3d of the unfrozen stages in training mode): the raw convolution on the HIP kernel, then
@@ -140,13 +166,16 @@ class NonLocal3d(nn.Module):
     """mmcv.cnn.NonLocal3d (mmcv 1.x `_NonLocalNd`), the configuration TRACE uses
     (i3d_nl_dot_product_...py:15-19: sub_sample=True, use_scale=False,
     mode='dot_product', BN on conv_out).  Source not vendored in the reference:
-    restated from mmcv's published behaviour (parity unpinned)."""
+    restated from mmcv's published behaviour (parity unpinned).
+    mode='embedded_gaussian' (mmcv's default) is softmax attention of every position over the (pooled) positions, with
+    use_scale divided by sqrt(inter_channels); it runs on ops.attention and needs inter_channels % 8 == 0, <= 512."""
 
     def __init__(self, in_channels, reduction=2, use_scale=True, conv_cfg=None, norm_cfg=None,
                  mode='embedded_gaussian', sub_sample=False, **kwargs):
         super().__init__()
-        if mode != 'dot_product':
-            raise NotImplementedError("only mode='dot_product' (TRACE's configuration) is built")
+        if mode not in ('dot_product', 'embedded_gaussian'):
+            raise NotImplementedError("only mode='dot_product' (TRACE's configuration) and 'embedded_gaussian' are built")
+        self.mode = mode
         self.in_channels = in_channels
         self.inter_channels = max(in_channels // reduction, 1)
         self.use_scale = use_scale
@@ -167,6 +196,9 @@ class NonLocal3d(nn.Module):
     def _conv(self, m):
         return m[0] if isinstance(m, nn.Sequential) else m
 
+    def _scale(self):
+        return self.inter_channels ** -0.5 if self.use_scale else 1.0
+
     def forward(self, x):
         n = x.size(0)
         c = self.inter_channels
@@ -174,14 +206,14 @@ class NonLocal3d(nn.Module):
         theta_x = self.theta(x).view(n, c, -1).permute(0, 2, 1)
         phi_x = self.phi(x).view(n, c, -1)
         pw = torch.matmul(theta_x, phi_x)
-        pw = pw / pw.shape[-1]
+        pw = torch.softmax(pw * self._scale(), -1) if self.mode == 'embedded_gaussian' else pw / pw.shape[-1]
         y = torch.matmul(pw, g_x).permute(0, 2, 1).contiguous().reshape(n, c, *x.size()[2:])
         return x + self.conv_out(y)
 
     def run_train(self, x):
         """The block under autograd: the four 1x1x1 convs and the two products (S = phi^T g per clip, y = theta S / N_kv -
-        dot_product mode has no softmax) and all their gradients on the HIP kernels (trace_amd/autograd.py); the
-        (1,2,2) max-pool of phi / g and the per-clip transposes are torch ops."""
+        dot_product mode has no softmax; embedded_gaussian: one attention over all clips) and all their gradients on the
+        HIP kernels (trace_amd/autograd.py); the (1,2,2) max-pool of phi / g and the per-clip transposes are torch ops."""
         from . import autograd as tag
         N, T, H, W, C = x.shape
         c = self.inter_channels
@@ -193,6 +225,9 @@ class NonLocal3d(nn.Module):
             pool = lambda t: F.max_pool3d(t.permute(0, 4, 1, 2, 3), (1, 2, 2)).permute(0, 2, 3, 4, 1)
             phi, g = pool(phi), pool(g)
         nkv = phi.shape[1] * phi.shape[2] * phi.shape[3]
+        if self.mode == 'embedded_gaussian':
+            y = tag.attention(theta.view(N, nq, 1, c), phi.reshape(N, nkv, 1, c), g.reshape(N, nkv, 1, c), self._scale())
+            return x + self.conv_out.run_train(y.view(N, T, H, W, c), relu=False)
         nkp = (nkv + 7) // 8 * 8
         phiT = F.pad(phi.reshape(N, nkv, c).transpose(1, 2), (0, nkp - nkv))      # (N, c, nkp): zero columns add nothing
         gT = F.pad(g.reshape(N, nkv, c).transpose(1, 2), (0, nkp - nkv))
@@ -216,12 +251,24 @@ class NonLocal3d(nn.Module):
         nq = T * H * W
         if self._tpg is not None and self._tpg[2] != _PACK_EPOCH[0]:
             self._tpg = None
+        if self.mode == 'embedded_gaussian':
+            # theta | phi | g as few launches, attention reads its operands as strided columns of their outputs
+            w, b = self._tpg_packed()
+            if self.sub_sample:
+                theta = ops.conv3d(x, w[:c], b[:c], (1, 1, 1)).view(N, nq, 1, c)
+                pg = ops.maxpool3d(ops.conv3d(x, w[c:], b[c:], (1, 1, 1)), (1, 2, 2), (1, 2, 2)).view(N, -1, 1, 2 * c)
+            else:
+                tpg = ops.conv3d(x, w, b, (1, 1, 1)).view(N, nq, 1, 3 * c)
+                theta, pg = tpg[..., :c], tpg[..., c:]
+            phi, g = pg[..., :c], pg[..., c:]
+            y = ops.attention(theta, phi, g, self._scale())
+            return self.conv_out.run(y.view(N, T, H, W, c), residual=x, relu=False)
         if self.sub_sample and c % 64 == 0:
             # theta|phi|g in one launch, then ONE kernel pools phi / g and lays them out for the products
             w, b = self._tpg_packed()
             tpg = ops.conv3d(x, w, b, (1, 1, 1))
             theta = tpg.view(N, nq, 3 * c)[:, :, :c]
-            if self.reassociate:
+            if self.reassociate and not self.conv_out.with_gn:
                 # dot_product mode has no softmax, so (theta phi^T / N_kv) g = theta (phi^T g / N_kv): the
                 # (N_q x N_kv) pairwise map is never formed (5x fewer FLOPs at 32f 224^2, no 39 MB intermediate),
                 # and conv_out folds into the per-clip (c x c) matrix:  x + conv_out(y) = x + theta (W_out S^T)^T + b
@@ -307,8 +354,9 @@ class Bottleneck3d(nn.Module):
         second output of the same launch - its bf16 rounding, which is what the next convs read as their operand; the
         f32 twin travels as `out._res32`.  Only conv OPERANDS are rounded to bf16 then, never the running sum."""
         ds = self.downsample
-        f32 = self.res_f32 and not pool_t2
-        fusable = (self.fuse_downsample and ds is not None and tuple(ds.conv.stride) == (1, 1, 1) and tuple(ds.conv.kernel_size) == (1, 1, 1)
+        gn = self.conv3.with_gn or (ds is not None and ds.with_gn)   # nothing of a GroupNorm folds into a GEMM
+        f32 = self.res_f32 and not pool_t2 and not gn
+        fusable = (self.fuse_downsample and ds is not None and not gn and tuple(ds.conv.stride) == (1, 1, 1) and tuple(ds.conv.kernel_size) == (1, 1, 1)
                    and x.shape[-1] % 64 == 0 and self.conv3.conv.in_channels % 64 == 0 and not pool_t2)
         if fusable:
             # relu(conv3(h) + downsample(x)) as ONE GEMM over [h | x] with weights [W3 | Wd]: the downsample output is
@@ -463,9 +511,12 @@ class ResNet3d(nn.Module):
             kt, kh, kw = self.conv1_kernel
             kwp = (kw + 1) // 2 * 2  # even number of pixels: kwp*CP % 8 == 0
             w, b = self.conv1.conv.weight.detach().float(), None
-            bn = self.conv1.bn
-            scale = bn.weight.detach().float() / torch.sqrt(bn.running_var.float() + bn.eps)
-            b = bn.bias.detach().float() - bn.running_mean.float() * scale
+            if self.conv1.with_gn:
+                scale, b = torch.ones(w.shape[0], device=w.device), torch.zeros(w.shape[0], device=w.device)
+            else:
+                bn = self.conv1.bn
+                scale = bn.weight.detach().float() / torch.sqrt(bn.running_var.float() + bn.eps)
+                b = bn.bias.detach().float() - bn.running_mean.float() * scale
             w = w * scale.view(-1, 1, 1, 1, 1)
             wp = torch.zeros((w.shape[0], kt, kh, kwp, self.CP), device=w.device)
             wp[:, :, :, :kw, :w.shape[1]] = w.permute(0, 2, 3, 4, 1)
@@ -476,7 +527,8 @@ class ResNet3d(nn.Module):
     def _run_stem(self, x, in_ntchw):
         """conv1 + BN + ReLU + maxpool (resnet3d.py:795-796).  The pool's kernel_t is 1 with
         stride_t 2, so only every second conv1 frame is ever read: the stem runs with temporal
-        stride conv1_stride_t*pool1_stride_t and the pool with temporal stride 1."""
+        stride conv1_stride_t*pool1_stride_t and the pool with temporal stride 1.  The statistics of a GroupNorm run over all
+        conv1 frames: then every one is computed, and the pool skips."""
         u8 = x.dtype == torch.uint8   # decoded frames (N,T,H,W,C); `in_ntchw` does not apply
         if u8:
             N, T, H, W, C = x.shape
@@ -490,30 +542,35 @@ class ResNet3d(nn.Module):
         w, b, kwp = self._stem_weights()
         pt, ph, pw = (kt - 1) // 2, (kh - 1) // 2, (kw - 1) // 2
         T1 = (T + 2 * pt - kt) // self.conv1_stride_t + 1
-        To = (T1 - 1) // self.pool1_stride_t + 1
+        gn = self.conv1.with_gn
+        To = T1 if gn else (T1 - 1) // self.pool1_stride_t + 1
         Ho = (H + 2 * ph - kh) // 2 + 1
         Wo = (W + 2 * pw - kw) // 2 + 1
         need_w = (Wo - 1) * 2 + kwp  # padded width the contiguous runs must fit in
         pw1 = max(need_w - (W + pw), pw)
         if (W + pw + pw1) % 2:
             pw1 += 1
-        st = self.conv1_stride_t * self.pool1_stride_t
+        st = self.conv1_stride_t * (1 if gn else self.pool1_stride_t)
+
+        def norm_pool(y):
+            if gn:
+                return ops.maxpool3d(self.conv1._group_norm(y, True), (1, 3, 3), (self.pool1_stride_t, 2, 2), (0, 1, 1))
+            return ops.maxpool3d(y, (1, 3, 3), (1, 2, 2), (0, 1, 1))
         if u8:
             if not ((kt, kh, kw) == (5, 7, 7) and kwp == 8 and self.CP == 4 and w.shape[0] == 64 and Ho % 16 == 0 and Wo % 16 == 0):
                 raise RuntimeError("uint8 frames are taken by TRACE's stem shape only (5x7x7, 64 couts, output H, W multiples "
                                    "of 16); convert to the f32 clip for other stems")
             # (float)u8 - pixel_means[c] while the kernel fills its LDS patch (get_frames_blob, test_engine_rel.py:420-520)
-            y = ops.conv3d_stem_u8(x, self.pixel_means, w, b, st, (To, Ho, Wo))
-            return ops.maxpool3d(y, (1, 3, 3), (1, 2, 2), (0, 1, 1))
+            y = ops.conv3d_stem_u8(x, self.pixel_means, w, b, st, (To, Ho, Wo), relu=not gn)
+            return norm_pool(y)
         if (self.stem_from_f32 and (kt, kh, kw) == (5, 7, 7) and kwp == 8 and self.CP == 4 and w.shape[0] == 64 and
                 Ho % 16 == 0 and Wo % 16 == 0 and x.dtype == torch.float32):
             # the stem kernel converts the f32 clip while it fills its LDS patch: no padded bf16 copy of the clip
-            y = ops.conv3d_stem_f32(x, in_ntchw, w, b, st, (To, Ho, Wo))
-            return ops.maxpool3d(y, (1, 3, 3), (1, 2, 2), (0, 1, 1))
+            y = ops.conv3d_stem_f32(x, in_ntchw, w, b, st, (To, Ho, Wo), relu=not gn)
+            return norm_pool(y)
         xp = ops.clip_to_ndhwc(x, in_ntchw, self.CP, (pt, pt, ph, ph, pw, pw1))
-        y = ops.conv3d_stem(xp, w, b, kt, kh, kwp, (self.conv1_stride_t * self.pool1_stride_t, 2, 2), (To, Ho, Wo),
-                            alg_k=kt * kh * kw * C)
-        return ops.maxpool3d(y, (1, 3, 3), (1, 2, 2), (0, 1, 1))
+        y = ops.conv3d_stem(xp, w, b, kt, kh, kwp, (st, 2, 2), (To, Ho, Wo), relu=not gn, alg_k=kt * kh * kw * C)
+        return norm_pool(y)
 
     def forward_ndhwc(self, x, in_ntchw=False, stage_hook=None, stop_after=None, start_at=None):
         """x f32 (N,C,T,H,W) (or (N,T,C,H,W) with in_ntchw), or uint8 decoded frames (N,T,H,W,C) from which
