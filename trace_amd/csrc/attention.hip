@@ -37,7 +37,7 @@ struct AttnArgs {
   const int32_t *q_len, *kv_len;
   uint16_t *o, *dq, *dk, *dv;
   float* lse;     // written by the forward, read by the backward kernels
-  float* delta;   // (B, H, Nq), backward
+  float* ndelta;  // (B, H, Nq): -delta, written by the dq kernel for the dk / dv one
   float* part;    // partial results of the splits (null: one split)
   float2* part_ml;
   int pack;       // query heads whose rows share one row axis (1, or all heads of a key head)
@@ -45,51 +45,57 @@ struct AttnArgs {
   int tiles, splits;
 };
 
-// LDS image of a tile: rows of 2 D bytes in 16-byte chunks, chunk c of row r at position c ^ at_key(r).  The key makes
-// both reads of a tile conflict-free over the 64 banks: a fragment read takes one chunk of 16 consecutive rows (16
-// different positions; 8 positions x 2 half-lines where a row is 128 bytes), a transposed read takes a 32-byte pair of
-// chunks of 8 consecutive rows (8 different pairs).
+// LDS image of a tile: rows of 2 D bytes in 16-byte chunks, chunk c of row r at position c ^ at_key(r).  The key makes both
+// reads of a tile conflict-free over the 64 banks.  A fragment read (ds_read_b128) serves 16 lanes at a time: rows 0-3 and
+// 12-15 of one chunk with rows 4-11 of its neighbour (chunk ^ 1), so the key leaves bit 0 alone; a transposed read
+// (ds_read_b64_tr_b16) takes a 32-byte pair of chunks of 8 consecutive rows, whose keys differ in the bits above (rows of 64 /
+// 128 bytes: 4 / 2 of them share a 256-byte line, only the others need different keys).
+// Bits of a chunk index and of a row's offset do not overlap, so the address of any chunk is the lane's base ^ a constant.
 template <int D> __device__ __forceinline__ int at_key(int r) {
-  return D >= 128 ? (((r & 7) << 1) | ((r >> 3) & 1)) : ((((r >> 1) & 3) << 1) | ((r >> 3) & 1));
+  return D >= 128 ? (r & 7) << 1 : D == 64 ? ((r >> 1) & 3) << 1 : ((r >> 2) & 1) << 1;
 }
 template <int D> __device__ __forceinline__ int at_off(int r, int chunk) { return r * (2 * D) + ((chunk ^ at_key<D>(r)) << 4); }
 
 // One wave's share of the LDS-DMA of a ROWS x D tile (whole workgroup: NW waves).
 template <int D, int ROWS, int NW> struct AtLoader {
   static constexpr int CPR = D / 8;
-  static constexpr int N = ROWS * CPR / (64 * NW);
-  static_assert(ROWS * CPR % (64 * NW) == 0, "whole instructions per wave");
-  const char* p[N];
-  unsigned colok;   // bit j: this lane's chunk of load j lies inside head_dim
-  long long step;   // bytes between rows
-  __device__ __forceinline__ void init(const uint16_t* base, long long row_stride, int d, int wave, int lane) {
+  static constexpr int INST = ROWS * CPR / 64, N = INST < NW ? 1 : INST / NW;   // loads of 1 KiB: in all, per wave
+  static_assert(ROWS * CPR % 64 == 0 && (INST < NW || INST % NW == 0), "whole instructions per wave");
+  uint32_t off[N];   // bytes from the tile's first row (rows x stride stay below 2^31: at_check)
+  unsigned colok;    // bit j: this lane's chunk of load j lies inside head_dim
+  __device__ __forceinline__ void init(long long row_stride, int d, int wave, int lane) {
     colok = 0;
-    step = row_stride * 2;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int id = (j * NW + wave) * 64 + lane, row = id / CPR, c = (id % CPR) ^ at_key<D>(row);
-      p[j] = reinterpret_cast<const char*>(base) + row * step + c * 16;
+      off[j] = (uint32_t)(row * row_stride * 2 + c * 16);
       if (c * 8 < d) colok |= 1u << j;
     }
   }
-  // rows row0 .. row0 + ROWS - 1 of the operand; rows >= row_end read zeros
-  __device__ __forceinline__ void issue(char* lds, int row0, int row_end, int wave, int lane) const {
+  // `rows` rows from `base` (uniform); further rows and the columns behind head_dim (`d` of D) read zeros
+  __device__ __forceinline__ void issue(char* lds, const uint16_t* base, int rows, int d, int wave, int lane) const {
+    if (INST < NW && wave >= INST) return;
+    const char* b = reinterpret_cast<const char*>(base);
+    if (rows >= ROWS && d == D) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) glds16(b + off[j], lds + (j * NW + wave) * 1024);
+      return;
+    }
     const char* zero = reinterpret_cast<const char*>(g_at_zero);
-    const long long adv = row0 * step;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int row = ((j * NW + wave) * 64 + lane) / CPR;
-      const bool ok = ((colok >> j) & 1u) && row0 + row < row_end;
-      glds16(ok ? p[j] + adv : zero, lds + (j * NW + wave) * 1024);
+      const bool ok = ((colok >> j) & 1u) && row < rows;
+      glds16(ok ? b + off[j] : zero, lds + (j * NW + wave) * 1024);
     }
   }
 };
 
-// B operand: rows of a (rows x D) operand as columns of the product, read straight from memory (16 bytes per lane)
-template <int D> __device__ __forceinline__ void at_load_cols(at_s8 (&f)[D / 32], const uint16_t* row, bool ok, int d, int g) {
+// B operand: a row of an operand as column of the product, 8 columns from 32 (kc0 + kc) + 8 g, straight from memory
+template <int KC> __device__ __forceinline__ void at_load_cols(at_s8 (&f)[KC], const uint16_t* row, bool ok, int kc0, int d, int g) {
 #pragma unroll
-  for (int kc = 0; kc < D / 32; ++kc) {
-    const int c = kc * 32 + g * 8;
+  for (int kc = 0; kc < KC; ++kc) {
+    const int c = (kc0 + kc) * 32 + g * 8;
     f[kc] = (ok && c < d) ? *reinterpret_cast<const at_s8*>(row + c) : at_s8{0, 0, 0, 0, 0, 0, 0, 0};
   }
 }
@@ -103,17 +109,21 @@ __device__ __forceinline__ at_s8 at_pack8(const at_f4& a, const at_f4& b) {
   return o.v;
 }
 
-// A operand of the summing product: rows r0 + {4 g .. 4 g + 3} and r0 + 16 + {..} of the tile (k), columns 16 dt + (lane & 15) (m)
-template <int D> __device__ __forceinline__ at_s8 at_tr(const char* tile, int r0, int dt, int lane) {
+// Lane bases of the two kinds of reads inside a tile (bytes); the tile's own offset is added before a chunk is selected.
+// rows: row lane & 15, chunk g;  selecting 32-column block kc: ^ kc << 6, rows 16 st ..: + st * 32 D
+template <int D> __device__ __forceinline__ int at_row_base(int lane) { return at_off<D>(lane & 15, lane >> 4); }
+// transposed: row 4 g + q, 8-byte half of the chunk pair; selecting columns 16 dt ..: ^ dt << 5, 16 rows further: + 32 D
+template <int D> __device__ __forceinline__ int at_tr_base(int lane) {
   const int g = lane >> 4, q = (lane >> 2) & 3, pq = lane & 3;
-  const int row = r0 + 4 * g + q, chunk = 2 * dt + (pq >> 1), half = (pq & 1) * 8;
-  const at_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_s4*)(tile + at_off<D>(row, chunk) + half));
-  const at_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_s4*)(tile + at_off<D>(row + 16, chunk) + half));
-  return at_s8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  return at_off<D>(4 * g + q, pq >> 1) + (pq & 1) * 8;
 }
-// A operand of a scoring product: rows r0 + (lane & 15), 8 columns from 32 kc + 8 g
-template <int D> __device__ __forceinline__ at_s8 at_row(const char* tile, int r0, int kc, int lane) {
-  return *reinterpret_cast<const at_s8*>(tile + at_off<D>(r0 + (lane & 15), kc * 4 + (lane >> 4)));
+__device__ __forceinline__ at_s8 at_row(const char* smem, int at) { return *reinterpret_cast<const at_s8*>(smem + at); }
+// A operand of the summing product: rows {4 g .. 4 g + 3} and {16 + 4 g ..} from `at` on (k), 16 columns (m = lane & 15)
+template <int D> __device__ __forceinline__ at_s8 at_tr(const char* smem, int at) {
+  typedef __attribute__((address_space(3))) at_s4* lp;
+  const at_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(smem + at));
+  const at_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(smem + at + 32 * D));
+  return at_s8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 }
 
 __device__ __forceinline__ at_f4 at_mfma(const at_s8& a, const at_s8& b, const at_f4& c) {
@@ -135,18 +145,58 @@ __device__ __forceinline__ void at_store4(uint16_t* dst, float a, float b, float
   *reinterpret_cast<uint2*>(dst) = o;
 }
 
+// s[st][nt] (16-row tiles of a staged tile x 16 columns) += rows . columns over the wave's KC 32-column blocks
+template <int D, int ST, int NT, int KC>
+__device__ __forceinline__ void at_score(const char* smem, int at, const at_s8 (&f)[NT][KC], at_f4 (&s)[ST][NT]) {
+#pragma unroll
+  for (int kc = 0; kc < KC; ++kc) {
+#pragma unroll
+    for (int st = 0; st < ST; ++st) {
+      const at_s8 a = at_row(smem, (at ^ (kc << 6)) + st * 32 * D);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[st][nt] = at_mfma(a, f[nt][kc], s[st][nt]);
+    }
+  }
+}
+
+// DW waves of a row group hold partial scores over their share of head_dim: every one gets the sum, added in wave order
+// (equal bits in all of them).  Each wave's scores pass through its own part of the exchange buffer; the caller has a barrier
+// between the last reads of one exchange and the next.
+template <int ST, int NT, int DW>
+__device__ __forceinline__ void at_exchange(char* xbuf, int wave, int lane, at_f4 (&s)[ST][NT]) {
+  constexpr int REG = ST * NT * 1024;
+  char* mine = xbuf + wave * REG + lane * 16;
+#pragma unroll
+  for (int st = 0; st < ST; ++st)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<at_f4*>(mine + (st * NT + nt) * 1024) = s[st][nt];
+  ring_barrier();
+  const int wd = wave % DW;
+  const char* group = xbuf + (wave - wd) * REG + lane * 16;
+#pragma unroll
+  for (int st = 0; st < ST; ++st)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      at_f4 t = *reinterpret_cast<const at_f4*>(group + (st * NT + nt) * 1024);
+#pragma unroll
+      for (int o = 1; o < DW; ++o) t += *reinterpret_cast<const at_f4*>(group + o * REG + (st * NT + nt) * 1024);
+      s[st][nt] = t;
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------------------
-// Forward.  A workgroup owns NW * NT * 16 query rows of one (batch, head); with few query rows the rows of all heads that
-// share a key head form one row axis (`pack`), so the keys are read once for them.  Key tiles of BN rows; `splits`
-// workgroups share the keys of a row tile and leave (max, sum, unnormalised out) for attn_combine_kernel.
+// Forward.  A row group of DW waves owns NT * 16 query rows of one (batch, head), each wave D / DW columns of head_dim; a
+// workgroup is NW / DW groups.  With few query rows the rows of all heads that share a key head form one row axis (`pack`), so
+// the keys are read once for them.  Key tiles of BN rows; `splits` workgroups share the keys of a row tile and leave (max, sum,
+// unnormalised out) for attn_combine_kernel.
 // ---------------------------------------------------------------------------------------------------------------
-template <int D, int NT, int NW, int BN>
-__global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs p) {
-  constexpr int TR = NW * NT * 16, KC = D / 32, DT = D / 16, ST = BN / 16;
+template <int D, int NT, int NW, int DW, int BN>
+__global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) {
+  constexpr int TR = NW / DW * NT * 16, KC = D / 32 / DW, DT = D / 16 / DW, ST = BN / 16;
   constexpr int TILE = BN * D * 2;
-  extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of [K tile][V tile]
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of [K tile][V tile], exchange buffer
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wd = wave % DW, wr = wave / DW;
   const int u = at_unit(blockIdx.x, gridDim.x);
   int tile = u % p.tiles;
   const int unit = (u / p.tiles) % p.units, b = u / p.tiles / p.units;
@@ -160,7 +210,7 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs p) {
   int wmin = 0x7fffffff, wmax = 0;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int r = tile * TR + (wave * NT + nt) * 16 + (lane & 15);
+    const int r = tile * TR + (wr * NT + nt) * 16 + (lane & 15);
     const int hh = p.pack > 1 ? r / p.Nq : 0;
     row_h[nt] = unit * p.pack + hh;
     row_i[nt] = r < nrows ? r - hh * p.Nq : -1;
@@ -168,7 +218,7 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs p) {
     lim[nt] = !ok ? 0 : p.causal ? min(max(row_i[nt] + diff + 1, 0), kvlen) : kvlen;
     if (lim[nt] > 0) wmin = min(wmin, lim[nt]);
     wmax = max(wmax, lim[nt]);
-    at_load_cols<D>(qf[nt], p.q + b * p.sq[0] + (ok ? row_i[nt] : 0) * p.sq[1] + (ok ? row_h[nt] : 0) * p.sq[2], ok, p.D, g);
+    at_load_cols<KC>(qf[nt], p.q + b * p.sq[0] + (ok ? row_i[nt] : 0) * p.sq[1] + (ok ? row_h[nt] : 0) * p.sq[2], ok, wd * KC, p.D, g);
   }
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
@@ -189,8 +239,16 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs p) {
   const int t0 = min((int)blockIdx.y * per, ntile), t1 = min(t0 + per, ntile);
 
   AtLoader<D, BN, NW> lk, lv;
-  lk.init(p.k + b * p.sk[0] + hk * p.sk[2], p.sk[1], p.D, wave, lane);
-  lv.init(p.v + b * p.sv[0] + hk * p.sv[2], p.sv[1], p.D, wave, lane);
+  lk.init(p.sk[1], p.D, wave, lane);
+  lv.init(p.sv[1], p.D, wave, lane);
+  const uint16_t* kb = p.k + b * p.sk[0] + hk * p.sk[2];
+  const uint16_t* vb = p.v + b * p.sv[0] + hk * p.sv[2];
+  auto issue = [&](int t) {
+    const int st = ((t - t0) & 1) * (2 * TILE), k0 = t * BN;
+    lk.issue(smem + st, kb + k0 * p.sk[1], kend - k0, p.D, wave, lane);
+    lv.issue(smem + st + TILE, vb + k0 * p.sv[1], kend - k0, p.D, wave, lane);
+  };
+  const int row_at = at_row_base<D>(lane) ^ (wd * KC << 6), tr_at = (at_tr_base<D>(lane) ^ (wd * DT << 5)) + TILE;
 
   const float c = p.scale * AT_LOG2E;
   at_f4 acc[DT][NT];
@@ -202,34 +260,20 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs p) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
   }
-  if (t0 < t1) {
-    lk.issue(smem, t0 * BN, kend, wave, lane);
-    lv.issue(smem + TILE, t0 * BN, kend, wave, lane);
-  }
+  if (t0 < t1) issue(t0);
   for (int t = t0; t < t1; ++t) {
     wait_vmcnt<0>();
     ring_barrier();   // tile t landed for every wave; every wave is done reading the other stage
-    const char* kt = smem + ((t - t0) & 1) * (2 * TILE);
-    const char* vt = kt + TILE;
-    if (t + 1 < t1) {
-      char* nx = smem + ((t + 1 - t0) & 1) * (2 * TILE);
-      lk.issue(nx, (t + 1) * BN, kend, wave, lane);
-      lv.issue(nx + TILE, (t + 1) * BN, kend, wave, lane);
-    }
-    const int key0 = t * BN;
-    if (key0 >= wmax) continue;   // no row of this wave sees these keys
+    const int stage = ((t - t0) & 1) * (2 * TILE), key0 = t * BN;
+    if (t + 1 < t1) issue(t + 1);
+    if (DW == 1 && key0 >= wmax) continue;   // no row of this wave sees these keys
     at_f4 s[ST][NT];
 #pragma unroll
-    for (int st = 0; st < ST; ++st) {
+    for (int st = 0; st < ST; ++st)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) s[st][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc) {
-        const at_s8 a = at_row<D>(kt, st * 16, kc, lane);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[st][nt] = at_mfma(a, qf[nt][kc], s[st][nt]);
-      }
-    }
+    at_score<D>(smem, row_at + stage, qf, s);
+    if constexpr (DW > 1) at_exchange<ST, NT, DW>(smem + 4 * TILE, wave, lane, s);
     if (key0 + BN > wmin) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -267,15 +311,15 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs p) {
       }
       // probabilities are rounded to bf16 for the product only (relative 2^-8 each, averaged over the row); their sum is not
 #pragma unroll
-      for (int kb = 0; kb < BN / 32; ++kb) pf[kb][nt] = at_pack8(s[2 * kb][nt], s[2 * kb + 1][nt]);
+      for (int kk = 0; kk < BN / 32; ++kk) pf[kk][nt] = at_pack8(s[2 * kk][nt], s[2 * kk + 1][nt]);
     }
 #pragma unroll
-    for (int kb = 0; kb < BN / 32; ++kb)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const at_s8 a = at_tr<D>(vt, kb * 32, dt, lane);
+      for (int kk = 0; kk < BN / 32; ++kk) {
+        const at_s8 a = at_tr<D>(smem, ((tr_at + stage) ^ (dt << 5)) + kk * 64 * D);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, pf[kb][nt], acc[dt][nt]);
+        for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, pf[kk][nt], acc[dt][nt]);
       }
   }
   const bool split = p.splits > 1;
@@ -289,19 +333,21 @@ __global__ __launch_bounds__(64 * NW) void attn_fwd_kernel(const AttnArgs p) {
     const long long row = ((long long)b * p.H + row_h[nt]) * p.Nq + row_i[nt];
     if (split) {
       const long long rows = (long long)p.B * p.H * p.Nq, at = blockIdx.y * rows + row;
-      if (g == 0) p.part_ml[at] = any ? make_float2(m[nt] * c, sum) : make_float2(-INFINITY, 0.f);
+      if (g == 0 && wd == 0) p.part_ml[at] = any ? make_float2(m[nt] * c, sum) : make_float2(-INFINITY, 0.f);
       if (!any) continue;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        if (16 * dt + 4 * g < p.D) *reinterpret_cast<at_f4*>(p.part + at * p.D + 16 * dt + 4 * g) = acc[dt][nt];
+      for (int dt = 0; dt < DT; ++dt) {
+        const int d = 16 * (wd * DT + dt) + 4 * g;
+        if (d < p.D) *reinterpret_cast<at_f4*>(p.part + at * p.D + d) = acc[dt][nt];
+      }
       continue;
     }
-    if (g == 0 && p.lse) p.lse[row] = any ? (m[nt] * c + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
+    if (g == 0 && wd == 0 && p.lse) p.lse[row] = any ? (m[nt] * c + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
     const float inv = any ? 1.f / sum : 0.f;
     uint16_t* o = p.o + (((long long)b * p.Nq + row_i[nt]) * p.H + row_h[nt]) * p.D;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const int d = 16 * dt + 4 * g;
+      const int d = 16 * (wd * DT + dt) + 4 * g;
       if (d < p.D) {
         if (any) at_store4(o + d, acc[dt][nt][0] * inv, acc[dt][nt][1] * inv, acc[dt][nt][2] * inv, acc[dt][nt][3] * inv);
         else at_store4(o + d, 0.f, 0.f, 0.f, 0.f);
@@ -339,15 +385,17 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// dq (and delta).  The same walk as the forward's over key tiles of 32, with two scoring products (q k^T and dout v^T).
+// dq (and delta).  The same walk as the forward's over key tiles of 32, with two scoring products (q k^T and dout v^T); the
+// second one starts from -delta instead of zero.
 // ---------------------------------------------------------------------------------------------------------------
-template <int D, int NT, int NW>
-__global__ __launch_bounds__(64 * NW) void attn_bwd_q_kernel(const AttnArgs p) {
-  constexpr int BN = 32, TR = NW * NT * 16, KC = D / 32, DT = D / 16;
+template <int D, int NT, int NW, int DW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p) {
+  constexpr int BN = 32, TR = NW / DW * NT * 16, KC = D / 32 / DW, DT = D / 16 / DW;
   constexpr int TILE = BN * D * 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wd = wave % DW, wr = wave / DW;
+  char* xbuf = smem + 4 * TILE;
   const int u = at_unit(blockIdx.x, gridDim.x);
   int tile = u % p.tiles;
   const int h = (u / p.tiles) % p.H, b = u / p.tiles / p.H;
@@ -356,25 +404,25 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_q_kernel(const AttnArgs p) {
   const int qlen = at_len(p.q_len, b, p.Nq), kvlen = at_len(p.kv_len, b, p.Nk), diff = kvlen - qlen;
 
   int row_i[NT], lim[NT];
-  float lse2[NT], delta[NT];
+  float lse2[NT], ndelta[NT];
   at_s8 qf[NT][KC], df[NT][KC];
   int wmin = 0x7fffffff, wmax = 0;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int i = tile * TR + (wave * NT + nt) * 16 + (lane & 15);
+    const int i = tile * TR + (wr * NT + nt) * 16 + (lane & 15);
     row_i[nt] = i;
     const bool ok = i < qlen;
     lim[nt] = !ok ? 0 : p.causal ? min(max(i + diff + 1, 0), kvlen) : kvlen;
     if (lim[nt] > 0) wmin = min(wmin, lim[nt]);
     wmax = max(wmax, lim[nt]);
     const int ii = ok ? i : 0;
-    at_load_cols<D>(qf[nt], p.q + b * p.sq[0] + ii * p.sq[1] + h * p.sq[2], ok, p.D, g);
-    at_load_cols<D>(df[nt], p.dout + b * p.sdo[0] + ii * p.sdo[1] + h * p.sdo[2], ok, p.D, g);
+    at_load_cols<KC>(qf[nt], p.q + b * p.sq[0] + ii * p.sq[1] + h * p.sq[2], ok, wd * KC, p.D, g);
+    at_load_cols<KC>(df[nt], p.dout + b * p.sdo[0] + ii * p.sdo[1] + h * p.sdo[2], ok, wd * KC, p.D, g);
     const uint16_t* orow = p.out + (((long long)b * p.Nq + ii) * p.H + h) * p.D;
     float sum = 0.f;
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
-      const int cc = kc * 32 + g * 8;
+      const int cc = (wd * KC + kc) * 32 + g * 8;
       if (ok && cc < p.D) {
         const at_s8 ov = *reinterpret_cast<const at_s8*>(orow + cc);
 #pragma unroll
@@ -383,11 +431,25 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_q_kernel(const AttnArgs p) {
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    delta[nt] = sum;
-    const long long row = ((long long)b * p.H + h) * p.Nq + ii;
-    lse2[nt] = ok ? p.lse[row] * AT_LOG2E : 0.f;
-    if (ok && g == 0 && blockIdx.y == 0) p.delta[row] = sum;
+    ndelta[nt] = -sum;
+    lse2[nt] = ok ? p.lse[((long long)b * p.H + h) * p.Nq + ii] * AT_LOG2E : 0.f;
   }
+  if constexpr (DW > 1) {   // the waves' shares of head_dim
+    float* xs = reinterpret_cast<float*>(xbuf);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) xs[(wave * NT + nt) * 64 + lane] = ndelta[nt];
+    ring_barrier();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float sum = 0.f;
+#pragma unroll
+      for (int o = 0; o < DW; ++o) sum += xs[((wave - wd + o) * NT + nt) * 64 + lane];
+      ndelta[nt] = sum;
+    }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+    if (row_i[nt] < qlen && g == 0 && wd == 0 && blockIdx.y == 0) p.ndelta[((long long)b * p.H + h) * p.Nq + row_i[nt]] = ndelta[nt];
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
     wmin = min(wmin, __shfl_xor(wmin, o));
@@ -403,44 +465,44 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_q_kernel(const AttnArgs p) {
   const int t0 = min((int)blockIdx.y * per, ntile), t1 = min(t0 + per, ntile);
 
   AtLoader<D, BN, NW> lk, lv;
-  lk.init(p.k + b * p.sk[0] + hk * p.sk[2], p.sk[1], p.D, wave, lane);
-  lv.init(p.v + b * p.sv[0] + hk * p.sv[2], p.sv[1], p.D, wave, lane);
+  lk.init(p.sk[1], p.D, wave, lane);
+  lv.init(p.sv[1], p.D, wave, lane);
+  const uint16_t* kb = p.k + b * p.sk[0] + hk * p.sk[2];
+  const uint16_t* vb = p.v + b * p.sv[0] + hk * p.sv[2];
+  auto issue = [&](int t) {
+    const int st = ((t - t0) & 1) * (2 * TILE), k0 = t * BN;
+    lk.issue(smem + st, kb + k0 * p.sk[1], kend - k0, p.D, wave, lane);
+    lv.issue(smem + st + TILE, vb + k0 * p.sv[1], kend - k0, p.D, wave, lane);
+  };
+  const int row_at = at_row_base<D>(lane) ^ (wd * KC << 6), tr_at = at_tr_base<D>(lane) ^ (wd * DT << 5);
   const float c = p.scale * AT_LOG2E;
   at_f4 acc[DT][NT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
-  if (t0 < t1) {
-    lk.issue(smem, t0 * BN, kend, wave, lane);
-    lv.issue(smem + TILE, t0 * BN, kend, wave, lane);
-  }
+  if (t0 < t1) issue(t0);
   for (int t = t0; t < t1; ++t) {
     wait_vmcnt<0>();
     ring_barrier();
-    const char* kt = smem + ((t - t0) & 1) * (2 * TILE);
-    const char* vt = kt + TILE;
-    if (t + 1 < t1) {
-      char* nx = smem + ((t + 1 - t0) & 1) * (2 * TILE);
-      lk.issue(nx, (t + 1) * BN, kend, wave, lane);
-      lv.issue(nx + TILE, (t + 1) * BN, kend, wave, lane);
-    }
-    const int key0 = t * BN;
-    if (key0 >= wmax) continue;
+    const int stage = ((t - t0) & 1) * (2 * TILE), key0 = t * BN;
+    if (t + 1 < t1) issue(t + 1);
+    if (DW == 1 && key0 >= wmax) continue;
     at_f4 s[2][NT], dp[2][NT];
 #pragma unroll
-    for (int st = 0; st < 2; ++st) {
+    for (int st = 0; st < 2; ++st)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[st][nt] = dp[st][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc) {
-        const at_s8 a = at_row<D>(kt, st * 16, kc, lane), av = at_row<D>(vt, st * 16, kc, lane);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[st][nt] = at_mfma(a, qf[nt][kc], s[st][nt]);
-          dp[st][nt] = at_mfma(av, df[nt][kc], dp[st][nt]);
-        }
+      for (int nt = 0; nt < NT; ++nt) {
+        const float d0 = DW == 1 || wd == 0 ? ndelta[nt] : 0.f;
+        s[st][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
+        dp[st][nt] = at_f4{d0, d0, d0, d0};
       }
+    at_score<D>(smem, row_at + stage, qf, s);
+    at_score<D>(smem, row_at + stage + TILE, df, dp);
+    if constexpr (DW > 1) {
+      at_exchange<2, NT, DW>(xbuf, wave, lane, s);
+      ring_barrier();
+      at_exchange<2, NT, DW>(xbuf, wave, lane, dp);
     }
     const bool mask = key0 + BN > wmin;
     at_s8 ds[NT];
@@ -452,13 +514,13 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_q_kernel(const AttnArgs p) {
         for (int r = 0; r < 4; ++r) {
           float pr = __builtin_amdgcn_exp2f(s[st][nt][r] * c - lse2[nt]);
           if (mask && key0 + st * 16 + 4 * g + r >= lim[nt]) pr = 0.f;
-          s[st][nt][r] = pr * (dp[st][nt][r] - delta[nt]);
+          s[st][nt][r] = pr * dp[st][nt][r];
         }
       ds[nt] = at_pack8(s[0][nt], s[1][nt]);
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const at_s8 a = at_tr<D>(kt, 0, dt, lane);
+      const at_s8 a = at_tr<D>(smem, (tr_at + stage) ^ (dt << 5));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, ds[nt], acc[dt][nt]);
     }
@@ -470,7 +532,7 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_q_kernel(const AttnArgs p) {
     const long long at = (((long long)b * p.Nq + row_i[nt]) * p.H + h) * p.D;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const int d = 16 * dt + 4 * g;
+      const int d = 16 * (wd * DT + dt) + 4 * g;
       if (d >= p.D) continue;
       const at_f4 a = any ? acc[dt][nt] : at_f4{0.f, 0.f, 0.f, 0.f};
       if (p.splits > 1)
@@ -482,21 +544,23 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_q_kernel(const AttnArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// dk and dv.  A workgroup owns NW * NT * 16 keys of one (batch, key head) - in registers as B operands - and walks the
+// dk and dv.  A workgroup owns NW / DW * NT * 16 keys of one (batch, key head) - in registers as B operands - and walks the
 // 32-row tiles of q and dout of every query head that reads it, so the gradients of shared heads are summed in a fixed order.
 // ---------------------------------------------------------------------------------------------------------------
-template <int D, int NT, int NW>
-__global__ __launch_bounds__(64 * NW) void attn_bwd_kv_kernel(const AttnArgs p) {
-  constexpr int BQ = 32, TK = NW * NT * 16, KC = D / 32, DT = D / 16;
-  constexpr int TILE = BQ * D * 2, STAGE = 2 * TILE + 256;   // [q][dout][32 lse, 32 delta]
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+template <int D, int NT, int NW, int DW>
+__global__ __launch_bounds__(64 * NW, D >= 512 ? 1 : 2) void attn_bwd_kv_kernel(const AttnArgs p) {
+  constexpr int BQ = 32, TK = NW / DW * NT * 16, KC = D / 32 / DW, DT = D / 16 / DW;
+  constexpr int TILE = BQ * D * 2;
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of [q][dout], two of [32 lse, 32 -delta], exchange
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wd = wave % DW, wr = wave / DW;
+  char* stats = smem + 4 * TILE;
+  char* xbuf = stats + 512;
   const int u = at_unit(blockIdx.x, gridDim.x);
   const int tile = u % p.tiles, hk = (u / p.tiles) % p.Hk, b = u / p.tiles / p.Hk;
   const int G = p.H / p.Hk;
   const int qlen = at_len(p.q_len, b, p.Nq), kvlen = at_len(p.kv_len, b, p.Nk), diff = kvlen - qlen;
-  const int key_first = tile * TK, wkey = key_first + wave * NT * 16;
+  const int key_first = tile * TK, wkey = key_first + wr * NT * 16;
 
   int key[NT];
   at_s8 kf[NT][KC], vf[NT][KC];
@@ -505,8 +569,8 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_kv_kernel(const AttnArgs p) 
     key[nt] = wkey + nt * 16 + (lane & 15);
     const bool ok = key[nt] < kvlen;
     const int kk = ok ? key[nt] : 0;
-    at_load_cols<D>(kf[nt], p.k + b * p.sk[0] + kk * p.sk[1] + hk * p.sk[2], ok, p.D, g);
-    at_load_cols<D>(vf[nt], p.v + b * p.sv[0] + kk * p.sv[1] + hk * p.sv[2], ok, p.D, g);
+    at_load_cols<KC>(kf[nt], p.k + b * p.sk[0] + kk * p.sk[1] + hk * p.sk[2], ok, wd * KC, p.D, g);
+    at_load_cols<KC>(vf[nt], p.v + b * p.sv[0] + kk * p.sv[1] + hk * p.sv[2], ok, wd * KC, p.D, g);
   }
   at_f4 ak[DT][NT], av[DT][NT];
 #pragma unroll
@@ -521,61 +585,62 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_kv_kernel(const AttnArgs p) 
   const int it0 = min((int)blockIdx.y * per, n_it), it1 = min(it0 + per, n_it);
 
   AtLoader<D, BQ, NW> lq, ld;
-  lq.init(p.q + b * p.sq[0] + (long long)hk * G * p.sq[2], p.sq[1], p.D, wave, lane);
-  ld.init(p.dout + b * p.sdo[0] + (long long)hk * G * p.sdo[2], p.sdo[1], p.D, wave, lane);
-  const long long head_q = p.sq[2] * 2, head_do = p.sdo[2] * 2;
-  const float* stat = (lane < 32 ? p.lse : p.delta) + ((long long)b * p.H + (long long)hk * G) * p.Nq;
+  lq.init(p.sq[1], p.D, wave, lane);
+  ld.init(p.sdo[1], p.D, wave, lane);
+  const uint16_t* qb = p.q + b * p.sq[0] + (long long)hk * G * p.sq[2];
+  const uint16_t* db = p.dout + b * p.sdo[0] + (long long)hk * G * p.sdo[2];
+  const float* stat = (lane < 32 ? p.lse : p.ndelta) + ((long long)b * p.H + (long long)hk * G) * p.Nq;
 
-  auto issue = [&](char* st, int it) {
-    const int hh = it / per_head, q0 = (qt0 + it - hh * per_head) * BQ;
-    AtLoader<D, BQ, NW> a = lq, d = ld;
-#pragma unroll
-    for (int j = 0; j < AtLoader<D, BQ, NW>::N; ++j) {
-      a.p[j] += hh * head_q;
-      d.p[j] += hh * head_do;
-    }
-    a.issue(st, q0, qlen, wave, lane);
-    d.issue(st + TILE, q0, qlen, wave, lane);
+  int head = 0, qt = 0;          // of the tile issued last
+  auto issue = [&](int it) {
+    const int par = (it - it0) & 1, q0 = qt * BQ;
+    lq.issue(smem + par * (2 * TILE), qb + head * p.sq[2] + q0 * p.sq[1], qlen - q0, p.D, wave, lane);
+    ld.issue(smem + par * (2 * TILE) + TILE, db + head * p.sdo[2] + q0 * p.sdo[1], qlen - q0, p.D, wave, lane);
     if (wave == 0) {
       const int i = q0 + (lane & 31);
-      const float* src = i < qlen ? stat + (long long)hh * p.Nq + i : reinterpret_cast<const float*>(g_at_zero);
-      __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(st + 2 * TILE), 4, 0, 0);
+      const float* src = i < qlen ? stat + (long long)head * p.Nq + i : reinterpret_cast<const float*>(g_at_zero);
+      __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(stats + par * 256), 4, 0, 0);
     }
   };
+  const int row_at = at_row_base<D>(lane) ^ (wd * KC << 6), tr_at = at_tr_base<D>(lane) ^ (wd * DT << 5);
   const float c = p.scale * AT_LOG2E;
-  if (it0 < it1) issue(smem, it0);
+  if (it0 < it1) {
+    head = it0 / per_head;
+    qt = qt0 + it0 - head * per_head;
+    issue(it0);
+  }
   for (int it = it0; it < it1; ++it) {
     wait_vmcnt<0>();
     ring_barrier();
-    const char* qt = smem + ((it - it0) & 1) * STAGE;
-    const char* dt_ = qt + TILE;
-    const float* st_ = reinterpret_cast<const float*>(qt + 2 * TILE);
-    if (it + 1 < it1) issue(smem + ((it + 1 - it0) & 1) * STAGE, it + 1);
-    const int q0 = (qt0 + it % per_head) * BQ;
-    if (p.causal && wkey > q0 + BQ - 1 + diff) continue;   // no key of this wave is seen
+    const int par = (it - it0) & 1, stage = par * (2 * TILE), q0 = qt * BQ;
+    if (++qt == nq) {
+      qt = qt0;
+      ++head;
+    }
+    if (it + 1 < it1) issue(it + 1);
+    if (DW == 1 && p.causal && wkey > q0 + BQ - 1 + diff) continue;   // no key of this wave is seen
     at_f4 s[2][NT], dp[2][NT];
+    const float* sp = reinterpret_cast<const float*>(stats + par * 256) + 4 * g;
+    at_f4 lse2[2];
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
+      lse2[st] = *reinterpret_cast<const at_f4*>(sp + st * 16) * AT_LOG2E;
+      const at_f4 nd = *reinterpret_cast<const at_f4*>(sp + 32 + st * 16);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[st][nt] = dp[st][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc) {
-        const at_s8 a = at_row<D>(qt, st * 16, kc, lane), ad = at_row<D>(dt_, st * 16, kc, lane);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[st][nt] = at_mfma(a, kf[nt][kc], s[st][nt]);
-          dp[st][nt] = at_mfma(ad, vf[nt][kc], dp[st][nt]);
-        }
+      for (int nt = 0; nt < NT; ++nt) {
+        s[st][nt] = at_f4{0.f, 0.f, 0.f, 0.f};
+        dp[st][nt] = DW == 1 || wd == 0 ? nd : at_f4{0.f, 0.f, 0.f, 0.f};
       }
+    }
+    at_score<D>(smem, row_at + stage, kf, s);
+    at_score<D>(smem, row_at + stage + TILE, vf, dp);
+    if constexpr (DW > 1) {
+      at_exchange<2, NT, DW>(xbuf, wave, lane, s);
+      ring_barrier();
+      at_exchange<2, NT, DW>(xbuf, wave, lane, dp);
     }
     const bool mask = q0 + BQ > qlen || wkey + NT * 16 > kvlen || (p.causal && wkey + NT * 16 - 1 > q0 + diff);
     at_s8 pf[NT], ds[NT];
-    at_f4 lse2[2], del[2];
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      lse2[st] = *reinterpret_cast<const at_f4*>(st_ + st * 16 + 4 * g) * AT_LOG2E;
-      del[st] = *reinterpret_cast<const at_f4*>(st_ + 32 + st * 16 + 4 * g);
-    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -586,17 +651,17 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_kv_kernel(const AttnArgs p) 
           const int i = q0 + st * 16 + 4 * g + r;
           if (mask && (i >= qlen || key[nt] >= kvlen || (p.causal && key[nt] > i + diff))) pr = 0.f;
           s[st][nt][r] = pr;
-          dp[st][nt][r] = pr * (dp[st][nt][r] - del[st][r]);
+          dp[st][nt][r] *= pr;
         }
       pf[nt] = at_pack8(s[0][nt], s[1][nt]);
       ds[nt] = at_pack8(dp[0][nt], dp[1][nt]);
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const at_s8 a = at_tr<D>(dt_, 0, dt, lane), aq = at_tr<D>(qt, 0, dt, lane);
+      const at_s8 ad = at_tr<D>(smem, (tr_at + stage + TILE) ^ (dt << 5)), aq = at_tr<D>(smem, (tr_at + stage) ^ (dt << 5));
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        av[dt][nt] = at_mfma(a, pf[nt], av[dt][nt]);
+        av[dt][nt] = at_mfma(ad, pf[nt], av[dt][nt]);
         ak[dt][nt] = at_mfma(aq, ds[nt], ak[dt][nt]);
       }
     }
@@ -608,7 +673,7 @@ __global__ __launch_bounds__(64 * NW) void attn_bwd_kv_kernel(const AttnArgs p) 
     const long long at = (((long long)b * p.Nk + key[nt]) * p.Hk + hk) * p.D;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const int d = 16 * dt + 4 * g;
+      const int d = 16 * (wd * DT + dt) + 4 * g;
       if (d >= p.D) continue;
       const at_f4 a = ak[dt][nt], w = av[dt][nt];
       if (p.splits > 1) {
@@ -645,10 +710,10 @@ struct AttnPlan {
 
 static inline size_t at_align(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Splits so that about two workgroups per CU exist, each with at least `min_iters` iterations of its loop.
-static int at_splits(long long groups, int iters, int min_iters) {
-  if (groups >= AT_CUS || groups <= 0) return 1;
-  long long s = (2 * AT_CUS + groups - 1) / groups;
+// Splits so that about `per_cu` workgroups per CU exist, each with at least `min_iters` iterations of its loop.
+static int at_splits(long long groups, int iters, int min_iters, int per_cu) {
+  if (groups <= 0 || 2 * groups > per_cu * AT_CUS) return 1;
+  long long s = (per_cu * AT_CUS + groups - 1) / groups;
   const long long most = iters / min_iters;
   if (s > most) s = most;
   if (s > 64) s = 64;
@@ -658,22 +723,23 @@ static int at_splits(long long groups, int iters, int min_iters) {
 static AttnPlan at_plan(const trace_attention_desc* d) {
   AttnPlan pl;
   const int hd = d->head_dim;
-  pl.D = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
+  pl.D = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
   const int G = d->heads / d->kv_heads;
-  // few query rows: all heads of a key head on one row axis, 16 rows per workgroup (its one wave streams the keys)
+  // few query rows: all heads of a key head on one row axis, 16 rows per workgroup (its one row group streams the keys)
   const bool small = (long long)d->q_rows * G <= 16;
   pl.pack = small ? G : 1;
   pl.units = d->heads / pl.pack;
-  pl.tile_rows = small ? 16 : pl.D <= 256 ? 128 : 64;
+  pl.tile_rows = small ? 16 : pl.D <= 128 ? 128 : 64;
   pl.tiles = ceil_div((long long)pl.pack * d->q_rows, pl.tile_rows);
-  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch * (small ? 1 : 1), ceil_div(d->k_rows, 32), 4);
-  const int bwd_rows = pl.D == 64 ? 256 : pl.D == 128 ? 128 : pl.D == 256 ? 64 : 64;
+  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch, ceil_div(d->k_rows, 32), 4, 2);
+  const int bwd_rows = pl.D <= 256 ? 128 : 64;
+  const int waves = d->causal ? 4 : 2;   // causal work is uneven: more, shorter workgroups
   pl.q_rows = bwd_rows;
   pl.q_tiles = ceil_div(d->q_rows, pl.q_rows);
-  pl.q_splits = at_splits((long long)pl.q_tiles * d->heads * d->batch, ceil_div(d->k_rows, 32), 4);
-  pl.k_rows = bwd_rows;
+  pl.q_splits = at_splits((long long)pl.q_tiles * d->heads * d->batch, ceil_div(d->k_rows, 32), 4, 2);
+  pl.k_rows = pl.D <= 256 ? 128 : 32;
   pl.k_tiles = ceil_div(d->k_rows, pl.k_rows);
-  pl.k_splits = at_splits((long long)pl.k_tiles * d->kv_heads * d->batch, ceil_div(d->q_rows, 32) * G, 4);
+  pl.k_splits = at_splits((long long)pl.k_tiles * d->kv_heads * d->batch, ceil_div(d->q_rows, 32) * G, 4, waves);
   return pl;
 }
 
@@ -688,6 +754,8 @@ static int at_check(const trace_attention_desc* d, const char* what) {
   TRACE_REQUIRE((long long)d->batch * d->heads * ((long long)d->q_rows + d->k_rows + 2) < (1ll << 31) - 1, "%s: too many rows", what);
   for (int i = 0; i < 3; ++i)
     TRACE_REQUIRE(((d->stride_q[i] | d->stride_k[i] | d->stride_v[i]) & 7) == 0, "%s: strides must be multiples of 8 elements", what);
+  for (long long st : {d->stride_q[1], d->stride_k[1], d->stride_v[1], d->stride_do[1]})   // 64-row tiles: 32-bit byte offsets
+    TRACE_REQUIRE(st >= 0 && st < (1ll << 24), "%s: row strides must be below 2^24 elements", what);
   return 0;
 }
 
@@ -717,22 +785,22 @@ static AttnArgs at_args(const trace_attention_desc* d, const uint16_t* q, const 
 
 static bool at_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int D, int NT, int NW, int BN> static int at_launch_fwd(const AttnArgs& a, hipStream_t st) {
-  const int lds = 2 * 2 * BN * D * 2;
-  TRACE_LDS_OPT_IN((attn_fwd_kernel<D, NT, NW, BN>), lds, "attention");
-  attn_fwd_kernel<D, NT, NW, BN><<<dim3((unsigned)a.tiles * a.units * a.B, a.splits), 64 * NW, lds, st>>>(a);
+template <int D, int NT, int NW, int DW, int BN> static int at_launch_fwd(const AttnArgs& a, hipStream_t st) {
+  const int lds = 4 * BN * D * 2 + (DW > 1 ? NW * (BN / 16) * NT * 1024 : 0);
+  TRACE_LDS_OPT_IN((attn_fwd_kernel<D, NT, NW, DW, BN>), lds, "attention");
+  attn_fwd_kernel<D, NT, NW, DW, BN><<<dim3((unsigned)a.tiles * a.units * a.B, a.splits), 64 * NW, lds, st>>>(a);
   return 0;
 }
-template <int D, int NT, int NW> static int at_launch_q(const AttnArgs& a, hipStream_t st) {
-  const int lds = 2 * 2 * 32 * D * 2;
-  TRACE_LDS_OPT_IN((attn_bwd_q_kernel<D, NT, NW>), lds, "attention backward");
-  attn_bwd_q_kernel<D, NT, NW><<<dim3((unsigned)a.tiles * a.H * a.B, a.splits), 64 * NW, lds, st>>>(a);
+template <int D, int NT, int NW, int DW> static int at_launch_q(const AttnArgs& a, hipStream_t st) {
+  const int lds = 4 * 32 * D * 2 + (DW > 1 ? NW * 2 * NT * 1024 : 0);
+  TRACE_LDS_OPT_IN((attn_bwd_q_kernel<D, NT, NW, DW>), lds, "attention backward");
+  attn_bwd_q_kernel<D, NT, NW, DW><<<dim3((unsigned)a.tiles * a.H * a.B, a.splits), 64 * NW, lds, st>>>(a);
   return 0;
 }
-template <int D, int NT, int NW> static int at_launch_kv(const AttnArgs& a, hipStream_t st) {
-  const int lds = 2 * (2 * 32 * D * 2 + 256);
-  TRACE_LDS_OPT_IN((attn_bwd_kv_kernel<D, NT, NW>), lds, "attention backward");
-  attn_bwd_kv_kernel<D, NT, NW><<<dim3((unsigned)a.tiles * a.Hk * a.B, a.splits), 64 * NW, lds, st>>>(a);
+template <int D, int NT, int NW, int DW> static int at_launch_kv(const AttnArgs& a, hipStream_t st) {
+  const int lds = 4 * 32 * D * 2 + 512 + (DW > 1 ? NW * 2 * NT * 1024 : 0);
+  TRACE_LDS_OPT_IN((attn_bwd_kv_kernel<D, NT, NW, DW>), lds, "attention backward");
+  attn_bwd_kv_kernel<D, NT, NW, DW><<<dim3((unsigned)a.tiles * a.Hk * a.B, a.splits), 64 * NW, lds, st>>>(a);
   return 0;
 }
 
@@ -777,17 +845,19 @@ extern "C" int trace_attention_fwd_bf16(const trace_attention_desc* d, const uin
   int rc = 0;
   if (pl.tile_rows == 16) {
     switch (pl.D) {
-      case 64: rc = at_launch_fwd<64, 1, 1, 32>(a, st); break;
-      case 128: rc = at_launch_fwd<128, 1, 1, 32>(a, st); break;
-      case 256: rc = at_launch_fwd<256, 1, 1, 32>(a, st); break;
-      default: rc = at_launch_fwd<512, 1, 1, 32>(a, st); break;
+      case 32: rc = at_launch_fwd<32, 1, 1, 1, 32>(a, st); break;
+      case 64: rc = at_launch_fwd<64, 1, 1, 1, 32>(a, st); break;
+      case 128: rc = at_launch_fwd<128, 1, 1, 1, 32>(a, st); break;
+      case 256: rc = at_launch_fwd<256, 1, 2, 2, 32>(a, st); break;
+      default: rc = at_launch_fwd<512, 1, 4, 4, 32>(a, st); break;
     }
   } else {
     switch (pl.D) {
-      case 64: rc = at_launch_fwd<64, 2, 4, 64>(a, st); break;
-      case 128: rc = at_launch_fwd<128, 2, 4, 64>(a, st); break;
-      case 256: rc = at_launch_fwd<256, 2, 4, 32>(a, st); break;
-      default: rc = at_launch_fwd<512, 1, 4, 32>(a, st); break;
+      case 32: rc = at_launch_fwd<32, 2, 4, 1, 64>(a, st); break;
+      case 64: rc = at_launch_fwd<64, 2, 4, 1, 64>(a, st); break;
+      case 128: rc = at_launch_fwd<128, 2, 4, 1, 64>(a, st); break;
+      case 256: rc = at_launch_fwd<256, 2, 4, 2, 32>(a, st); break;
+      default: rc = at_launch_fwd<512, 2, 8, 4, 32>(a, st); break;
     }
   }
   if (rc) return rc;
@@ -839,7 +909,7 @@ extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uin
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;
-  a.delta = reinterpret_cast<float*>(workspace);
+  a.ndelta = reinterpret_cast<float*>(workspace);
   a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + s.delta);
   hipStream_t st = (hipStream_t)stream;
   int rc = 0;
@@ -847,10 +917,11 @@ extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uin
     a.tiles = pl.q_tiles;
     a.splits = pl.q_splits;
     switch (pl.D) {
-      case 64: rc = at_launch_q<64, 4, 4>(a, st); break;
-      case 128: rc = at_launch_q<128, 2, 4>(a, st); break;
-      case 256: rc = at_launch_q<256, 1, 4>(a, st); break;
-      default: rc = at_launch_q<512, 1, 4>(a, st); break;
+      case 32: rc = at_launch_q<32, 2, 4, 1>(a, st); break;
+      case 64: rc = at_launch_q<64, 2, 4, 1>(a, st); break;
+      case 128: rc = at_launch_q<128, 2, 4, 1>(a, st); break;
+      case 256: rc = at_launch_q<256, 2, 8, 2>(a, st); break;
+      default: rc = at_launch_q<512, 2, 8, 4>(a, st); break;
     }
     if (rc) return rc;
     if (int e = check_launch("attention backward (dq)")) return e;
@@ -864,10 +935,11 @@ extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uin
     a.tiles = pl.k_tiles;
     a.splits = pl.k_splits;
     switch (pl.D) {
-      case 64: rc = at_launch_kv<64, 4, 4>(a, st); break;
-      case 128: rc = at_launch_kv<128, 2, 4>(a, st); break;
-      case 256: rc = at_launch_kv<256, 1, 4>(a, st); break;
-      default: rc = at_launch_kv<512, 1, 4>(a, st); break;
+      case 32: rc = at_launch_kv<32, 2, 4, 1>(a, st); break;
+      case 64: rc = at_launch_kv<64, 2, 4, 1>(a, st); break;
+      case 128: rc = at_launch_kv<128, 2, 4, 1>(a, st); break;
+      case 256: rc = at_launch_kv<256, 2, 8, 2>(a, st); break;
+      default: rc = at_launch_kv<512, 2, 4, 4>(a, st); break;
     }
     if (rc) return rc;
     if (int e = check_launch("attention backward (dk, dv)")) return e;
