@@ -552,7 +552,9 @@ int trace_upload_slots(const void* pinned, size_t slot_bytes, unsigned* counter,
  *   q_len, kv_len int32 DEVICE arrays (batch) or NULL = all rows; values are clamped to 0 .. q_rows / k_rows
  *   causal        query i sees key j <= i + kv_len - q_len (the last query sees every key)
  *   out[i] = sum_j softmax_j(scale q_i . k_j) v_j over the keys j < kv_len that i sees; lse[i] = log sum_j exp(scale q_i . k_j)
- *            (batch, heads, q_rows) f32.  Rows i >= q_len and rows that see no key: out = 0, lse = -inf, no gradient.
+ *            (batch, heads, q_rows) f32, may be NULL.  out_rest, NULL or like out: what rounding `out` to bf16 lost, itself in
+ *            bf16, with the probabilities carried to 16 bits more - the backward pass needs it, because dout . out is the
+ *            difference it takes from every dout . v.  Rows i >= q_len and rows that see no key: out = 0, lse = -inf, no gradient.
  *            Operand rows behind q_len / kv_len are never read; rows of dk / dv behind kv_len and of dq behind q_len are
  *            written as zeros.  Keys and values in front of kv_len have to be finite also where `causal` hides them.
  * Nothing is summed by atomics: equal calls give equal bits.  workspace: trace_attention_{fwd,bwd}_workspace_bytes(desc)
@@ -567,11 +569,13 @@ typedef struct {
 } trace_attention_desc;
 size_t trace_attention_fwd_workspace_bytes(const trace_attention_desc* desc);
 int trace_attention_fwd_bf16(const trace_attention_desc* desc, const uint16_t* q, const uint16_t* k, const uint16_t* v,
-                             uint16_t* out, float* lse, void* workspace, size_t workspace_bytes, trace_stream_t stream);
+                             uint16_t* out, float* lse, uint16_t* out_rest, void* workspace, size_t workspace_bytes,
+                             trace_stream_t stream);
 size_t trace_attention_bwd_workspace_bytes(const trace_attention_desc* desc);
 int trace_attention_bwd_bf16(const trace_attention_desc* desc, const uint16_t* q, const uint16_t* k, const uint16_t* v,
-                             const uint16_t* out, const float* lse, const uint16_t* dout, uint16_t* dq, uint16_t* dk,
-                             uint16_t* dv, void* workspace, size_t workspace_bytes, trace_stream_t stream);
+                             const uint16_t* out, const float* lse, const uint16_t* out_rest, const uint16_t* dout,
+                             uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace, size_t workspace_bytes,
+                             trace_stream_t stream);
 
 /* Group normalisation + activation over channels-last maps x (N, P, C), P = product of the positions, contiguous:
  *   z = (x - mean) / sqrt(var + eps) * gamma + beta with the mean / biased variance of each sample's groups of C / G

@@ -3,7 +3,8 @@
 Tolerances are bounds per element, from the roundings the kernels make (u = eps / 2 of bf16 = 2^-8, relative):
   out   u |out|  (the result)  +  u sum_j P_j |v_j|  (P is rounded to bf16 for the product)
   dv    u |dv| + u sum_i P_ij |dout_i|
-  dS    u |dS|  (rounded for the product)  +  P_ij e_i,  e_i = sum_d |dout_id| (error of out_id): delta is formed from the rounded out
+  dS    u |dS|  (rounded for the product)  +  P_ij e_i,  e_i = sum_d |dout_id| 2 u^2 (|out_id| + sum_j P_j |v_jd|): delta is formed
+        from out + rest, each rounding of which leaves u of what the first one left
   dq    u |dq| + scale sum_j (bound of dS)_ij |k_j|;  dk likewise over i
 and what 32-bit sums lose: a score is off by (D + 2) 2^-24 sum_d |q_d k_d| scale, its exponential by that, by the rounding of
 lse (2^-23 |lse|) and by the hardware's exp2 (2^-20 taken), relative to P; dP by (D + 2) 2^-24 sum_d |dout_d v_d|; sums over
@@ -67,7 +68,8 @@ def reference(q, k, v, do, scale, causal, ln):
             dp = dd @ vv.t()
             delta = (dd * o).sum(1, keepdim=True)
             ds = P * (dp - delta)
-            e_ds = P * ((dd.abs() * e_o).sum(1, keepdim=True) + (D + 2) * F * (dd.abs() @ vv.abs().t() + (dd.abs() * o.abs()).sum(1, keepdim=True)))
+            e_fine = 2 * U * U * (o.abs() + A) + (p_rel[:, None] + lk * F) * A
+            e_ds = P * ((dd.abs() * e_fine).sum(1, keepdim=True) + (D + 2) * F * (dd.abs() @ vv.abs().t() + (dd.abs() * o.abs()).sum(1, keepdim=True)))
             e_ds = e_ds + (p_rel[:, None] + U) * (ds.abs() + e_ds)
             e_p = (p_rel[:, None] + U) * P
             dq = scale * ds @ kk
@@ -117,19 +119,23 @@ def run_case(B, Nq, Nk, H, Hk, D, causal, mode, scale=None, spread=1.0, seed=0, 
         kw["q_len"] = torch.tensor([a for a, _ in ln], dtype=torch.int32, device=DEV)
     if mode != "none":
         kw["kv_len"] = torch.tensor([b for _, b in ln], dtype=torch.int32, device=DEV)
-    out, lse = ops.attention(q, k, v, return_lse=True, **kw)
+    out, lse, rest = ops.attention(q, k, v, for_backward=True, **kw)
     check(out, ref["out"], "out")
     dead = lse_ref == -math.inf
     lse_c = lse.double().cpu()
     assert torch.equal(lse_c == -math.inf, dead)
     assert float(((lse_c - lse_ref).abs() - lse_bnd)[~dead].max() if (~dead).any() else 0.0) <= 0.0
-    dq, dk, dv = ops.attention_backward(do, q, k, v, out, lse, **kw)
+    dq, dk, dv = ops.attention_backward(do, q, k, v, out, lse, rest, **kw)
     check(dv, ref["dv"], "dv")
     check(dq, ref["dq"], "dq")
     check(dk, ref["dk"], "dk")
+    # the forward pass alone: one product, its probabilities rounded
+    plain, plain_lse = ops.attention(q, k, v, return_lse=True, **kw)
+    check(plain, ref["out"], "out alone")
+    assert torch.equal(plain_lse, lse)
     # equal calls, equal bits
-    out2, lse2 = ops.attention(q, k, v, return_lse=True, **kw)
-    again = ops.attention_backward(do, q, k, v, out2, lse2, **kw)
+    out2, lse2, rest2 = ops.attention(q, k, v, for_backward=True, **kw)
+    again = ops.attention_backward(do, q, k, v, out2, lse2, rest2, **kw)
     assert torch.equal(out, out2) and all(torch.equal(a, b) for a, b in zip((dq, dk, dv), again))
 
 
@@ -177,14 +183,14 @@ def test_peaked_and_flat_rows(spread, scale):
 def test_no_keys_no_rows():
     from trace_amd import ops
     q, k, v, do = (t.to(DEV) for t in make(2, 5, 0, 2, 1, 64, 3))
-    out, lse = ops.attention(q, k, v, return_lse=True)
-    assert not out.any() and (lse == -math.inf).all()
-    dq, dk, dv = ops.attention_backward(do, q, k, v, out, lse)
+    out, lse, rest = ops.attention(q, k, v, for_backward=True)
+    assert not out.any() and not rest.any() and (lse == -math.inf).all()
+    dq, dk, dv = ops.attention_backward(do, q, k, v, out, lse, rest)
     assert not dq.any() and dk.shape == k.shape and dv.shape == v.shape
     q, k, v, do = (t.to(DEV) for t in make(2, 0, 5, 2, 1, 64, 3))
-    out, lse = ops.attention(q, k, v, return_lse=True)
+    out, lse, rest = ops.attention(q, k, v, for_backward=True)
     assert out.shape == q.shape and lse.shape == (2, 2, 0)
-    dq, dk, dv = ops.attention_backward(do, q, k, v, out, lse)
+    dq, dk, dv = ops.attention_backward(do, q, k, v, out, lse, rest)
     assert not dk.any() and not dv.any()
     q, k, v, do = (t.to(DEV) for t in make(0, 4, 5, 2, 1, 64, 3))
     assert ops.attention(q, k, v).shape == (0, 4, 2, 64)
@@ -297,8 +303,8 @@ def test_refusals():
     big = torch.zeros((1, 4, 1, 520), dtype=torch.bfloat16, device=DEV)
     with pytest.raises(RuntimeError):
         ops.attention(big, big, big)
-    out, lse = ops.attention(q, k, v, return_lse=True)
-    for args in ((do[:, :4], q, k, v, out, lse), (do, q, k, v, out[:, :4], lse), (do, q, k, v, out, lse[:, :2]),
-                 (do, q, k, v, out.float(), lse), (do, q, k, v, out, lse.double())):
+    out, lse, rest = ops.attention(q, k, v, for_backward=True)
+    for args in ((do[:, :4], q, k, v, out, lse, rest), (do, q, k, v, out[:, :4], lse, rest), (do, q, k, v, out, lse[:, :2], rest),
+                 (do, q, k, v, out.float(), lse, rest), (do, q, k, v, out, lse.double(), rest), (do, q, k, v, out, lse, rest[:1])):
         with pytest.raises(RuntimeError):
             ops.attention_backward(*args)

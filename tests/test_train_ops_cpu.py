@@ -66,22 +66,23 @@ def test_attention_entry_refuses():
                dict(head_dim=68), dict(head_dim=520), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
                dict(strides=(8, 4, 8)), dict(batch=1 << 15, heads=1 << 10, kv_heads=1, q_rows=1 << 10)):
         d = desc(**kw)
-        assert l.trace_attention_fwd_bf16(d, ok, ok, ok, ok, ok, ok, 1 << 40, None) != 0, kw
-        assert l.trace_attention_bwd_bf16(d, ok, ok, ok, ok, ok, ok, ok, ok, ok, ok, 1 << 40, None) != 0, kw
+        assert l.trace_attention_fwd_bf16(d, ok, ok, ok, ok, ok, None, ok, 1 << 40, None) != 0, kw
+        assert l.trace_attention_bwd_bf16(d, *[ok] * 10, ok, 1 << 40, None) != 0, kw
         assert l.trace_attention_fwd_workspace_bytes(d) == 0
     d = desc()
     for i in (0, 1, 2, 3):
         for v in (None, ok + 8):
-            a = [ok] * 5
+            a = [ok] * 6
             a[i] = v
             assert l.trace_attention_fwd_bf16(d, *a, ok, 1 << 30, None) != 0
-    for i in range(9):
-        a = [ok] * 9
+    assert l.trace_attention_fwd_bf16(d, ok, ok, ok, ok, ok, ok + 8, ok, 1 << 30, None) != 0
+    for i in range(10):
+        a = [ok] * 10
         a[i] = None
         assert l.trace_attention_bwd_bf16(d, *a, ok, 1 << 30, None) != 0
-    assert l.trace_attention_bwd_bf16(d, *[ok] * 9, ok, 16, None) != 0            # workspace too small
-    assert l.trace_attention_bwd_bf16(d, *[ok] * 9, None, 1 << 30, None) != 0
+    assert l.trace_attention_bwd_bf16(d, *[ok] * 10, ok, 16, None) != 0            # workspace too small
+    assert l.trace_attention_bwd_bf16(d, *[ok] * 10, None, 1 << 30, None) != 0
     long_keys = desc(q_rows=1, k_rows=100000)
     assert l.trace_attention_fwd_workspace_bytes(long_keys) > 0
-    assert l.trace_attention_fwd_bf16(long_keys, ok, ok, ok, ok, ok, ok, 0, None) != 0
-    assert l.trace_attention_fwd_bf16(desc(batch=0), None, None, None, None, None, None, 0, None) == 0
+    assert l.trace_attention_fwd_bf16(long_keys, ok, ok, ok, ok, ok, None, ok, 0, None) != 0
+    assert l.trace_attention_fwd_bf16(desc(batch=0), *[None] * 7, 0, None) == 0

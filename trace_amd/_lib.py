@@ -94,9 +94,9 @@ SIGNATURES = {
                                   ctypes.POINTER(TreeGruWeights), c_int, P, P, P, c_size_t, P]),
     "trace_tree_gru_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "trace_attention_fwd_workspace_bytes": (c_size_t, [ctypes.POINTER(AttentionDesc)]),
-    "trace_attention_fwd_bf16": (c_int, [ctypes.POINTER(AttentionDesc), P, P, P, P, P, P, c_size_t, P]),
+    "trace_attention_fwd_bf16": (c_int, [ctypes.POINTER(AttentionDesc), P, P, P, P, P, P, P, c_size_t, P]),
     "trace_attention_bwd_workspace_bytes": (c_size_t, [ctypes.POINTER(AttentionDesc)]),
-    "trace_attention_bwd_bf16": (c_int, [ctypes.POINTER(AttentionDesc), P, P, P, P, P, P, P, P, P, P, c_size_t, P]),
+    "trace_attention_bwd_bf16": (c_int, [ctypes.POINTER(AttentionDesc), P, P, P, P, P, P, P, P, P, P, P, c_size_t, P]),
     "trace_group_norm_workspace_bytes": (c_size_t, [c_int, c_longlong, c_int, c_int, c_int]),
     "trace_group_norm_act_bf16": (c_int, [P, c_int, c_longlong, c_int, c_int, P, P, c_float, c_int, P, P, P, c_size_t, P]),
     "trace_group_norm_act_f32": (c_int, [P, c_int, c_longlong, c_int, c_int, P, P, c_float, c_int, P, P, P, c_size_t, P]),

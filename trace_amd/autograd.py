@@ -148,22 +148,25 @@ def gemm_nt(x, w, bias=None, relu=False):
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, causal, q_len, kv_len):
-        out, lse = ops.attention(q, k, v, scale, causal, q_len, kv_len, return_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse, q_len, kv_len)
+        out, lse, rest = ops.attention(q, k, v, scale, causal, q_len, kv_len, for_backward=True)
+        ctx.save_for_backward(q, k, v, out, lse, rest, q_len, kv_len)
         ctx.cfg = (scale, causal)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        q, k, v, out, lse, q_len, kv_len = ctx.saved_tensors
-        grads = ops.attention_backward(gout.to(torch.bfloat16), q, k, v, out, lse, *ctx.cfg, q_len, kv_len)
+        q, k, v, out, lse, rest, q_len, kv_len = ctx.saved_tensors
+        grads = ops.attention_backward(gout.to(torch.bfloat16), q, k, v, out, lse, rest, *ctx.cfg, q_len, kv_len)
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 4
 
 
 def attention(q, k, v, scale=None, causal=False, q_len=None, kv_len=None):
     """Differentiable ops.attention (same arguments); gradients reach q, k and v.  Kept for the backward pass: the operands,
-    the output and one f32 per row - the probabilities are recomputed."""
+    the output, what its rounding lost (another bf16 tensor like it) and one f32 per row - the probabilities are recomputed.
+    Without a gradient to come it is ops.attention itself."""
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return ops.attention(q, k, v, scale, causal, q_len, kv_len)
     return _Attention.apply(q, k, v, scale, bool(causal), q_len, kv_len)
 
 

@@ -30,12 +30,12 @@ constexpr float AT_LOG2E = 1.4426950408889634f, AT_LN2 = 0.6931471805599453f;
 constexpr int AT_CUS = 256;
 
 struct AttnArgs {
-  const uint16_t *q, *k, *v, *out, *dout;
+  const uint16_t *q, *k, *v, *out, *rest, *dout;
   long long sq[3], sk[3], sv[3], sdo[3];   // elements between batches / rows / heads
   int B, Nq, Nk, H, Hk, D, causal;
   float scale;
   const int32_t *q_len, *kv_len;
-  uint16_t *o, *dq, *dk, *dv;
+  uint16_t *o, *o_rest, *dq, *dk, *dv;
   float* lse;     // written by the forward, read by the backward kernels
   float* ndelta;  // (B, H, Nq): -delta, written by the dq kernel for the dk / dv one
   float* part;    // partial results of the splits (null: one split)
@@ -109,6 +109,17 @@ __device__ __forceinline__ at_s8 at_pack8(const at_f4& a, const at_f4& b) {
   return o.v;
 }
 
+// bf16 of what at_pack8 lost
+__device__ __forceinline__ at_s8 at_lost8(const at_f4& a, const at_f4& b, const at_s8& packed) {
+  at_f4 x, y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    x[r] = a[r] - bf16_to_f32((uint16_t)packed[r]);
+    y[r] = b[r] - bf16_to_f32((uint16_t)packed[4 + r]);
+  }
+  return at_pack8(x, y);
+}
+
 // Lane bases of the two kinds of reads inside a tile (bytes); the tile's own offset is added before a chunk is selected.
 // rows: row lane & 15, chunk g;  selecting 32-column block kc: ^ kc << 6, rows 16 st ..: + st * 32 D
 template <int D> __device__ __forceinline__ int at_row_base(int lane) { return at_off<D>(lane & 15, lane >> 4); }
@@ -143,6 +154,17 @@ __device__ __forceinline__ void at_store4(uint16_t* dst, float a, float b, float
   o.x = pack_bf16x2(a, b);
   o.y = pack_bf16x2(c, d);
   *reinterpret_cast<uint2*>(dst) = o;
+}
+
+// the result, and what its rounding lost
+template <bool FINE> __device__ __forceinline__ void at_store_out(const AttnArgs& p, long long at, const at_f4& v) {
+  uint2 o;
+  o.x = pack_bf16x2(v[0], v[1]);
+  o.y = pack_bf16x2(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p.o + at) = o;
+  if constexpr (FINE)
+    at_store4(p.o_rest + at, v[0] - bf16_to_f32((uint16_t)o.x), v[1] - bf16_to_f32((uint16_t)(o.x >> 16)),
+              v[2] - bf16_to_f32((uint16_t)o.y), v[3] - bf16_to_f32((uint16_t)(o.y >> 16)));
 }
 
 // s[st][nt] (16-row tiles of a staged tile x 16 columns) += rows . columns over the wave's KC 32-column blocks
@@ -189,8 +211,12 @@ __device__ __forceinline__ void at_exchange(char* xbuf, int wave, int lane, at_f
 // workgroup is NW / DW groups.  With few query rows the rows of all heads that share a key head form one row axis (`pack`), so
 // the keys are read once for them.  Key tiles of BN rows; `splits` workgroups share the keys of a row tile and leave (max, sum,
 // unnormalised out) for attn_combine_kernel.
+// The probabilities are rounded to bf16 for the product (2^-9 each on average, averaged over a row), which is as much as the
+// result's own rounding.  FINE (a forward pass that a backward pass follows): a second product adds what that rounding lost, and
+// what rounding the result loses is written as well.  delta = dout . out enters every dS = P (dout v^T - delta): with the
+// plain out, half of the error of dq and dk came from it (relative 2.6 - 3.1e-3 against 2.3e-3).
 // ---------------------------------------------------------------------------------------------------------------
-template <int D, int NT, int NW, int DW, int BN>
+template <int D, int NT, int NW, int DW, int BN, bool FINE>
 __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) {
   constexpr int TR = NW / DW * NT * 16, KC = D / 32 / DW, DT = D / 16 / DW, ST = BN / 16;
   constexpr int TILE = BN * D * 2;
@@ -283,7 +309,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
           for (int r = 0; r < 4; ++r)
             if (key0 + st * 16 + 4 * g + r >= lim[nt]) s[st][nt][r] = -INFINITY;
     }
-    at_s8 pf[BN / 32][NT];
+    at_s8 pf[BN / 32][NT], pl[BN / 32][NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float mx = m[nt];
@@ -309,9 +335,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[dt][nt] *= alpha;
       }
-      // probabilities are rounded to bf16 for the product only (relative 2^-8 each, averaged over the row); their sum is not
 #pragma unroll
-      for (int kk = 0; kk < BN / 32; ++kk) pf[kk][nt] = at_pack8(s[2 * kk][nt], s[2 * kk + 1][nt]);
+      for (int kk = 0; kk < BN / 32; ++kk) {   // the sum above is not rounded
+        pf[kk][nt] = at_pack8(s[2 * kk][nt], s[2 * kk + 1][nt]);
+        if constexpr (FINE) pl[kk][nt] = at_lost8(s[2 * kk][nt], s[2 * kk + 1][nt], pf[kk][nt]);
+      }
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -319,7 +347,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
       for (int kk = 0; kk < BN / 32; ++kk) {
         const at_s8 a = at_tr<D>(smem, ((tr_at + stage) ^ (dt << 5)) + kk * 64 * D);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, pf[kk][nt], acc[dt][nt]);
+        for (int nt = 0; nt < NT; ++nt) {
+          acc[dt][nt] = at_mfma(a, pf[kk][nt], acc[dt][nt]);
+          if constexpr (FINE) acc[dt][nt] = at_mfma(a, pl[kk][nt], acc[dt][nt]);
+        }
       }
   }
   const bool split = p.splits > 1;
@@ -344,20 +375,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
     }
     if (g == 0 && wd == 0 && p.lse) p.lse[row] = any ? (m[nt] * c + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
     const float inv = any ? 1.f / sum : 0.f;
-    uint16_t* o = p.o + (((long long)b * p.Nq + row_i[nt]) * p.H + row_h[nt]) * p.D;
+    const long long o = (((long long)b * p.Nq + row_i[nt]) * p.H + row_h[nt]) * p.D;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const int d = 16 * (wd * DT + dt) + 4 * g;
-      if (d < p.D) {
-        if (any) at_store4(o + d, acc[dt][nt][0] * inv, acc[dt][nt][1] * inv, acc[dt][nt][2] * inv, acc[dt][nt][3] * inv);
-        else at_store4(o + d, 0.f, 0.f, 0.f, 0.f);
-      }
+      if (d < p.D) at_store_out<FINE>(p, o + d, any ? acc[dt][nt] * inv : at_f4{0.f, 0.f, 0.f, 0.f});
     }
   }
 }
 
 // out / lse of a row from its splits' (max, sum, unnormalised out), in split order; one thread per four columns
-__global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs p) {
+template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs p) {
   const int dq = p.D >> 2;
   const long long rows = (long long)p.B * p.H * p.Nq;
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -380,7 +408,7 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs p) {
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   const int i = (int)(row % p.Nq), h = (int)(row / p.Nq % p.H);
   const long long b = row / p.Nq / p.H;
-  at_store4(p.o + ((b * p.Nq + i) * p.H + h) * p.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  at_store_out<FINE>(p, ((b * p.Nq + i) * p.H + h) * p.D + d, o * inv);
   if (d == 0 && p.lse) p.lse[row] = sum > 0.f ? (mx + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
 }
 
@@ -418,15 +446,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
     const int ii = ok ? i : 0;
     at_load_cols<KC>(qf[nt], p.q + b * p.sq[0] + ii * p.sq[1] + h * p.sq[2], ok, wd * KC, p.D, g);
     at_load_cols<KC>(df[nt], p.dout + b * p.sdo[0] + ii * p.sdo[1] + h * p.sdo[2], ok, wd * KC, p.D, g);
-    const uint16_t* orow = p.out + (((long long)b * p.Nq + ii) * p.H + h) * p.D;
+    const long long orow = (((long long)b * p.Nq + ii) * p.H + h) * p.D;
     float sum = 0.f;
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
       const int cc = (wd * KC + kc) * 32 + g * 8;
       if (ok && cc < p.D) {
-        const at_s8 ov = *reinterpret_cast<const at_s8*>(orow + cc);
+        const at_s8 ov = *reinterpret_cast<const at_s8*>(p.out + orow + cc), rv = *reinterpret_cast<const at_s8*>(p.rest + orow + cc);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += bf16_to_f32((uint16_t)ov[e]) * bf16_to_f32((uint16_t)df[nt][kc][e]);
+        for (int e = 0; e < 8; ++e)
+          sum += (bf16_to_f32((uint16_t)ov[e]) + bf16_to_f32((uint16_t)rv[e])) * bf16_to_f32((uint16_t)df[nt][kc][e]);
       }
     }
     sum += __shfl_xor(sum, 16);
@@ -787,8 +816,14 @@ static bool at_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <int D, int NT, int NW, int DW, int BN> static int at_launch_fwd(const AttnArgs& a, hipStream_t st) {
   const int lds = 4 * BN * D * 2 + (DW > 1 ? NW * (BN / 16) * NT * 1024 : 0);
-  TRACE_LDS_OPT_IN((attn_fwd_kernel<D, NT, NW, DW, BN>), lds, "attention");
-  attn_fwd_kernel<D, NT, NW, DW, BN><<<dim3((unsigned)a.tiles * a.units * a.B, a.splits), 64 * NW, lds, st>>>(a);
+  const dim3 grid((unsigned)a.tiles * a.units * a.B, a.splits);
+  if (a.o_rest) {
+    TRACE_LDS_OPT_IN((attn_fwd_kernel<D, NT, NW, DW, BN, true>), lds, "attention");
+    attn_fwd_kernel<D, NT, NW, DW, BN, true><<<grid, 64 * NW, lds, st>>>(a);
+  } else {
+    TRACE_LDS_OPT_IN((attn_fwd_kernel<D, NT, NW, DW, BN, false>), lds, "attention");
+    attn_fwd_kernel<D, NT, NW, DW, BN, false><<<grid, 64 * NW, lds, st>>>(a);
+  }
   return 0;
 }
 template <int D, int NT, int NW, int DW> static int at_launch_q(const AttnArgs& a, hipStream_t st) {
@@ -820,17 +855,19 @@ extern "C" size_t trace_attention_fwd_workspace_bytes(const trace_attention_desc
 }
 
 extern "C" int trace_attention_fwd_bf16(const trace_attention_desc* d, const uint16_t* q, const uint16_t* k, const uint16_t* v,
-                                        uint16_t* out, float* lse, void* workspace, size_t workspace_bytes,
-                                        trace_stream_t stream) {
+                                        uint16_t* out, float* lse, uint16_t* out_rest, void* workspace,
+                                        size_t workspace_bytes, trace_stream_t stream) {
   if (int rc = at_check(d, "attention")) return rc;
   if (d->batch == 0 || d->q_rows == 0) return 0;
   TRACE_REQUIRE(q && out && (d->k_rows == 0 || (k && v)), "attention: null pointer");
-  TRACE_REQUIRE(at_aligned(q) && at_aligned(k) && at_aligned(v) && at_aligned(out), "attention: operands must be 16-byte aligned");
+  TRACE_REQUIRE(at_aligned(q) && at_aligned(k) && at_aligned(v) && at_aligned(out) && at_aligned(out_rest),
+                "attention: operands must be 16-byte aligned");
   const AttnPlan pl = at_plan(d);
   const size_t need = at_fwd_bytes(d, pl);
   TRACE_REQUIRE(workspace_bytes >= need && (!need || workspace), "attention: workspace of %zu bytes needed", need);
   AttnArgs a = at_args(d, q, k, v);
   a.o = out;
+  a.o_rest = out_rest;
   a.lse = lse;
   a.pack = pl.pack;
   a.units = pl.units;
@@ -863,7 +900,9 @@ extern "C" int trace_attention_fwd_bf16(const trace_attention_desc* d, const uin
   if (rc) return rc;
   if (int e = check_launch("attention")) return e;
   if (pl.splits > 1) {
-    attn_combine_kernel<<<ceil_div(rows * (d->head_dim / 4), 256), 256, 0, st>>>(a);
+    const int grid = ceil_div(rows * (d->head_dim / 4), 256);
+    if (out_rest) attn_combine_kernel<true><<<grid, 256, 0, st>>>(a);
+    else attn_combine_kernel<false><<<grid, 256, 0, st>>>(a);
     return check_launch("attention combine");
   }
   return 0;
@@ -887,15 +926,16 @@ extern "C" size_t trace_attention_bwd_workspace_bytes(const trace_attention_desc
 }
 
 extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uint16_t* q, const uint16_t* k, const uint16_t* v,
-                                        const uint16_t* out, const float* lse, const uint16_t* dout, uint16_t* dq, uint16_t* dk,
-                                        uint16_t* dv, void* workspace, size_t workspace_bytes, trace_stream_t stream) {
+                                        const uint16_t* out, const float* lse, const uint16_t* out_rest,
+                                        const uint16_t* dout, uint16_t* dq, uint16_t* dk, uint16_t* dv, void* workspace,
+                                        size_t workspace_bytes, trace_stream_t stream) {
   if (int rc = at_check(d, "attention backward")) return rc;
   for (int i = 0; i < 3; ++i)
     TRACE_REQUIRE((d->stride_do[i] & 7) == 0, "attention backward: strides must be multiples of 8 elements");
   if (d->batch == 0) return 0;
-  TRACE_REQUIRE(d->q_rows == 0 || (q && out && lse && dout && dq), "attention backward: null pointer");
+  TRACE_REQUIRE(d->q_rows == 0 || (q && out && lse && out_rest && dout && dq), "attention backward: null pointer");
   TRACE_REQUIRE(d->k_rows == 0 || (k && v && dk && dv), "attention backward: null pointer");
-  TRACE_REQUIRE(at_aligned(q) && at_aligned(k) && at_aligned(v) && at_aligned(out) && at_aligned(dout) && at_aligned(dq) &&
+  TRACE_REQUIRE(at_aligned(q) && at_aligned(k) && at_aligned(v) && at_aligned(out) && at_aligned(out_rest) && at_aligned(dout) && at_aligned(dq) &&
                     at_aligned(dk) && at_aligned(dv),
                 "attention backward: operands must be 16-byte aligned");
   const AttnPlan pl = at_plan(d);
@@ -904,6 +944,7 @@ extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uin
   TRACE_REQUIRE(workspace_bytes >= need && (!need || workspace), "attention backward: workspace of %zu bytes needed", need);
   AttnArgs a = at_args(d, q, k, v);
   a.out = out;
+  a.rest = out_rest;
   a.dout = dout;
   a.lse = const_cast<float*>(lse);
   a.dq = dq;

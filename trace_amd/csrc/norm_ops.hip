@@ -8,8 +8,8 @@
 //   * one workgroup per (sample, slab of whole groups) that keeps the slab in registers between the statistics and the
 //     result: everything is read once, one launch.  Taken where the slab fits (P rows of at least 64 contiguous bytes, <=
 //     GN_R 16-byte pieces per thread);
-//   * larger maps in two passes over (sample, chunk of rows): partial statistics, then the result from the merged
-//     ones; the second pass walks the chunks from the last to the first, so that it starts with what the caches still hold.
+//   * larger maps in two passes over (sample, chunk of rows), a small merge of the chunks' partial results between them; the
+//     second pass walks the chunks from the last to the first, so that it starts with what the caches still hold.
 // Statistics are merged as (count, mean, sum of squared deviations), never as sum of squares minus squared sum: a map whose
 // mean is far from zero loses nothing.  All sums in f32, in a fixed order.
 #include "common.h"
@@ -33,40 +33,54 @@ struct GnArgs {
   int N, C, G, Cg, P, act;
   float eps;
   int slab;             // groups per workgroup of the one-pass form
+  int pow2;             // its columns, and those of a group, are powers of two of whole accesses
   int rows, chunks;     // two-pass: rows per chunk
 };
 
-template <typename T, int V> struct GnVec;   // V elements of T, as loaded
-template <> struct GnVec<uint16_t, 8> { using type = uint4; };
-template <> struct GnVec<uint16_t, 4> { using type = uint2; };
-template <> struct GnVec<uint16_t, 2> { using type = uint32_t; };
-template <> struct GnVec<uint16_t, 1> { using type = uint16_t; };
-template <> struct GnVec<float, 4> { using type = float4; };
-template <> struct GnVec<float, 2> { using type = float2; };
-template <> struct GnVec<float, 1> { using type = float; };
+// V elements of T as loaded: bf16 as 32-bit words of two (one element alone: itself), f32 as they are
+template <typename T, int V> struct GnVec;
+template <> struct GnVec<uint16_t, 8> { typedef __attribute__((ext_vector_type(4))) uint32_t type; };
+template <> struct GnVec<uint16_t, 4> { typedef __attribute__((ext_vector_type(2))) uint32_t type; };
+template <> struct GnVec<uint16_t, 2> { typedef __attribute__((ext_vector_type(1))) uint32_t type; };
+template <> struct GnVec<uint16_t, 1> { typedef uint16_t type; };
+template <> struct GnVec<float, 4> { typedef __attribute__((ext_vector_type(4))) float type; };
+template <> struct GnVec<float, 2> { typedef __attribute__((ext_vector_type(2))) float type; };
+template <> struct GnVec<float, 1> { typedef __attribute__((ext_vector_type(1))) float type; };
 
+// bf16 pairs are taken apart by 32-bit operations where they are used: as 16-bit elements every one would hold a register
 template <typename T, int V> __device__ __forceinline__ void gn_unpack(const typename GnVec<T, V>::type& r, float (&f)[V]) {
-  T e[V];
-  memcpy(e, &r, sizeof(e));
+  if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if constexpr (std::is_same<T, float>::value) f[i] = e[i];
-    else f[i] = bf16_to_f32(e[i]);
+    for (int i = 0; i < V; ++i) f[i] = r[i];
+  } else if constexpr (V == 1) {
+    f[0] = bf16_to_f32(r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      f[2 * i] = __uint_as_float(r[i] << 16);
+      f[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+    }
   }
 }
 template <typename T, int V> __device__ __forceinline__ typename GnVec<T, V>::type gn_pack(const float (&f)[V]) {
-  T e[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if constexpr (std::is_same<T, float>::value) e[i] = f[i];
-    else e[i] = f32_to_bf16(f[i]);
-  }
   typename GnVec<T, V>::type r;
-  memcpy(&r, e, sizeof(e));
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = f[i];
+  } else if constexpr (V == 1) {
+    r = f32_to_bf16(f[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+  }
   return r;
 }
 
-__device__ __forceinline__ float gn_sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
+// between the rows of an unrolled loop: the compiler would otherwise unpack all of them at once, in as many registers
+__device__ __forceinline__ void gn_row_done() { __builtin_amdgcn_sched_barrier(0); }
+
+// hardware reciprocal (1 ulp): a correctly rounded division would cost more than the rest of the element
+__device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
 template <int V> __device__ __forceinline__ void gn_act(float (&z)[V], int act) {
   if (act & TRACE_EPI_RELU) {
@@ -126,6 +140,37 @@ template <int BT> __device__ __forceinline__ void gn_sum_cols(float* a, int nseg
   }
 }
 
+// Group sums of K values per thread where a slab's columns (SW, CVG of them to a group) are powers of two: butterflies over the
+// lane bits that do not tell groups apart, then one exchange between the waves.  Every thread gets the sums of its own group.
+template <int BT, int K> __device__ __forceinline__ void gn_group_sums(float (&v)[K], int SW, int CVG, float* red, int tid) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1)
+    if (o < CVG || o >= SW) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], o);
+    }
+  // column of a thread within the slab -> its group; a slab wider than a wave has several waves per row
+  const int groups = SW / CVG, g = (tid & (SW - 1)) / CVG, span = max(min(CVG, 64), 1);
+  if (((tid & 63) & (span - 1)) == 0 && (SW >= 64 || (tid & 63) < SW)) {
+    // one writer per (wave, group present in the wave)
+#pragma unroll
+    for (int k = 0; k < K; ++k) red[((tid >> 6) * groups + g) * K + k] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = 0.f;
+  for (int w = 0; w < BT / 64; ++w) {
+    // waves of a wide slab hold different columns: only those whose columns meet this group
+    if (SW > 64) {
+      const int first = (w * 64) & (SW - 1);
+      if (first / CVG > g || (first + 63) / CVG < g) continue;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += red[(w * groups + g) * K + k];
+  }
+  __syncthreads();
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // One pass: workgroup (slab of `slab` groups, sample).  Thread = one V-wide column of the slab, rows tid / SW + i RP.
 // ---------------------------------------------------------------------------------------------------------------
@@ -147,7 +192,7 @@ __global__ __launch_bounds__(GN_BT) void gn_fwd_slab_kernel(const GnArgs p) {
     if (on && row < p.P) raw[i] = *reinterpret_cast<const Raw*>(x + (long long)row * p.C);
   }
   const float inv = 1.f / ((float)p.P * (float)p.Cg);
-  float mean[V], s[V];
+  float mean[V], rstd[V], s[V];
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {   // the mean, then the squared deviations from it
 #pragma unroll
@@ -163,6 +208,20 @@ __global__ __launch_bounds__(GN_BT) void gn_fwd_slab_kernel(const GnArgs p) {
           s[v] += pass ? d * d : d;
         }
       }
+      gn_row_done();
+    }
+    if (p.pow2) {
+      float t[1] = {0.f};
+#pragma unroll
+      for (int v = 0; v < V; ++v) t[0] += s[v];
+      gn_group_sums<GN_BT, 1>(t, SW, p.Cg / V, red, tid);
+      const float r = pass ? 1.f / sqrtf(t[0] * inv + p.eps) : t[0] * inv;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (pass) rstd[v] = r;
+        else mean[v] = r;
+      }
+      continue;
     }
     if (on) {
 #pragma unroll
@@ -176,21 +235,26 @@ __global__ __launch_bounds__(GN_BT) void gn_fwd_slab_kernel(const GnArgs p) {
       dst[c] = pass ? 1.f / sqrtf(t + p.eps) : t;
     }
     __syncthreads();
-    if (!pass) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) mean[v] = on ? mu[col + v] : 0.f;
+    for (int v = 0; v < V; ++v) {
+      if (pass) rstd[v] = on ? rs[col + v] : 0.f;
+      else mean[v] = on ? mu[col + v] : 0.f;
     }
   }
-  for (int g = tid; g < p.slab; g += GN_BT) {
-    float* st = p.stats + 2 * ((long long)n * p.G + blockIdx.x * p.slab + g);
-    st[0] = mu[g * p.Cg];
-    st[1] = rs[g * p.Cg];
-  }
   if (!on) return;
+  if (r0 == 0) {   // the thread that holds a group's first channel
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if ((col + v) % p.Cg == 0) {
+        float* st = p.stats + 2 * ((long long)n * p.G + (c0 + col + v) / p.Cg);
+        st[0] = mean[v];
+        st[1] = rstd[v];
+      }
+  }
   float ga[V], be[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    ga[v] = rs[col + v] * (p.gamma ? p.gamma[c0 + col + v] : 1.f);
+    ga[v] = rstd[v] * (p.gamma ? p.gamma[c0 + col + v] : 1.f);
     be[v] = p.beta ? p.beta[c0 + col + v] : 0.f;
   }
   T* y = static_cast<T*>(p.out) + (long long)n * p.P * p.C + c0 + col;
@@ -205,6 +269,17 @@ __global__ __launch_bounds__(GN_BT) void gn_fwd_slab_kernel(const GnArgs p) {
       gn_act<V>(f, p.act);
       *reinterpret_cast<Raw*>(y + (long long)row * p.C) = gn_pack<T, V>(f);
     }
+    gn_row_done();
+  }
+}
+
+// a channel's sums of dz and dz xh in one sample: the parameters' gradients themselves if there is no other sample
+__device__ __forceinline__ void gn_channel_out(const GnArgs& p, int n, int c, float a, float b) {
+  if (p.N > 1) {
+    *reinterpret_cast<float2*>(p.csum + 2 * ((long long)n * p.C + c)) = make_float2(a, b);
+  } else {
+    if (p.dbeta) p.dbeta[c] = a;
+    if (p.dgamma) p.dgamma[c] = b;
   }
 }
 
@@ -257,34 +332,76 @@ __global__ __launch_bounds__(GN_BT) void gn_bwd_slab_kernel(const GnArgs p) {
         b[v] += d[v] * f[v];
       }
     }
+    gn_row_done();
   }
-  if (on) {
+  const float inv = 1.f / ((float)p.P * (float)p.Cg);
+  if (p.pow2) {
+    float t[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      ra[r0 * SC + col + v] = a[v];
-      rb[r0 * SC + col + v] = b[v];
+      t[0] += a[v] * ga[v];
+      t[1] += b[v] * ga[v];
+    }
+    gn_group_sums<GN_BT, 2>(t, SW, p.Cg / V, ra, tid);
+    // per channel: over the rows of a wave, then over the waves (of a slab as wide as a wave or wider there is nothing to add
+    // within one, and the waves of one column are SW / 64 apart)
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+      if (o >= SW) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          a[v] += __shfl_xor(a[v], o);
+          b[v] += __shfl_xor(b[v], o);
+        }
+      }
+    if ((tid & 63) < SW) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        ra[(tid & 63) * V + v + (tid >> 6) * (min(SW, 64) * V)] = a[v];
+        rb[(tid & 63) * V + v + (tid >> 6) * (min(SW, 64) * V)] = b[v];
+      }
+    }
+    __syncthreads();
+    const int per = min(SW, 64) * V, apart = max(SW / 64, 1);   // channels a wave holds, waves per row
+    for (int c = tid; c < SC; c += GN_BT) {
+      float sa = 0.f, sb = 0.f;
+      for (int w = c / per; w < GN_BT / 64; w += apart) {
+        sa += ra[w * per + c % per];
+        sb += rb[w * per + c % per];
+      }
+      gn_channel_out(p, n, c0 + c, sa, sb);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      a[v] = t[0] * inv;
+      b[v] = t[1] * inv;
+    }
+  } else {
+    if (on) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        ra[r0 * SC + col + v] = a[v];
+        rb[r0 * SC + col + v] = b[v];
+      }
+    }
+    gn_sum_rows<GN_BT>(ra, SC, RP, tid);
+    gn_sum_rows<GN_BT>(rb, SC, RP, tid);
+    for (int c = tid; c < SC; c += GN_BT) {   // per channel: kept for dgamma / dbeta; weighted: the group's sums
+      gn_channel_out(p, n, c0 + c, ra[c], rb[c]);
+      const float w = p.gamma ? p.gamma[c0 + c] : 1.f;
+      ra[c] *= w;
+      rb[c] *= w;
+    }
+    gn_sum_cols<GN_BT>(ra, p.slab, p.Cg, tid);
+    gn_sum_cols<GN_BT>(rb, p.slab, p.Cg, tid);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int g = on ? (col + v) / p.Cg * p.Cg : 0;
+      a[v] = ra[g] * inv;
+      b[v] = rb[g] * inv;
     }
   }
-  gn_sum_rows<GN_BT>(ra, SC, RP, tid);
-  gn_sum_rows<GN_BT>(rb, SC, RP, tid);
-  for (int c = tid; c < SC; c += GN_BT) {   // per channel: kept for dgamma / dbeta; weighted: the group's sums
-    float* cs = p.csum + 2 * ((long long)n * p.C + c0 + c);
-    cs[0] = ra[c];
-    cs[1] = rb[c];
-    const float w = p.gamma ? p.gamma[c0 + c] : 1.f;
-    ra[c] *= w;
-    rb[c] *= w;
-  }
-  gn_sum_cols<GN_BT>(ra, p.slab, p.Cg, tid);
-  gn_sum_cols<GN_BT>(rb, p.slab, p.Cg, tid);
   if (!on) return;
-  const float inv = 1.f / ((float)p.P * (float)p.Cg);
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int g = (col + v) / p.Cg * p.Cg;
-    a[v] = ra[g] * inv;
-    b[v] = rb[g] * inv;
-  }
   T* dx = static_cast<T*>(p.out) + base;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -303,6 +420,7 @@ __global__ __launch_bounds__(GN_BT) void gn_bwd_slab_kernel(const GnArgs p) {
       for (int v = 0; v < V; ++v) d[v] = (d[v] * ga[v] - a[v] - f[v] * b[v]) * rstd[v];
       *reinterpret_cast<Raw*>(dx + (long long)row * p.C) = gn_pack<T, V>(d);
     }
+    gn_row_done();
   }
 }
 
@@ -357,6 +475,7 @@ __global__ __launch_bounds__(GN_CT) void gn_stats_kernel(const GnArgs p) {
             gn_unpack<T, V>(raw[i], f);
 #pragma unroll
             for (int v = 0; v < V; ++v) s[v] += f[v];
+            gn_row_done();
           }
         const float kf = (float)k, ik = 1.f / kf, tot = cnt + kf, w = kf / tot;
 #pragma unroll
@@ -368,6 +487,7 @@ __global__ __launch_bounds__(GN_CT) void gn_stats_kernel(const GnArgs p) {
             gn_unpack<T, V>(raw[i], f);
 #pragma unroll
             for (int v = 0; v < V; ++v) q[v] += (f[v] - s[v]) * (f[v] - s[v]);
+            gn_row_done();
           }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -428,42 +548,27 @@ __global__ __launch_bounds__(GN_CT) void gn_stats_kernel(const GnArgs p) {
   }
 }
 
-// y of a chunk; every workgroup merges its sample's partial statistics itself (a launch less; chunks * G * 8 bytes of L2)
+// wave per (group, sample): the chunks' moments, each lane a strided list in order, then pairs of lanes -> stats
+__global__ __launch_bounds__(64) void gn_merge_kernel(const GnArgs p) {
+  const int lane = threadIdx.x, g = blockIdx.x, n = blockIdx.y;
+  GnMom m = {0.f, 0.f, 0.f};
+  for (int k = lane; k < p.chunks; k += 64) {
+    const float2 o = *reinterpret_cast<const float2*>(p.part + 2 * (((long long)n * p.chunks + k) * p.G + g));
+    m = gn_merge(m, {(float)min(p.rows, p.P - k * p.rows) * (float)p.Cg, o.x, o.y});
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const GnMom t = {__shfl_xor(m.n, o), __shfl_xor(m.mean, o), __shfl_xor(m.m2, o)};
+    m = (lane & o) ? gn_merge(t, m) : gn_merge(m, t);   // both lanes the same way round
+  }
+  if (lane == 0)
+    *reinterpret_cast<float2*>(p.stats + 2 * ((long long)n * p.G + g)) = make_float2(m.mean, 1.f / sqrtf(m.m2 / m.n + p.eps));
+}
+
 template <typename T, int V>
 __global__ __launch_bounds__(GN_CT) void gn_apply_kernel(const GnArgs p) {
   using Raw = typename GnVec<T, V>::type;
-  extern __shared__ float sm[];   // [C] scale, [C] shift, [G] mean, [G] rstd, [GN_CT] x 3 moments
-  float *sc = sm, *sh = sm + p.C, *mu = sh + p.C, *rs = mu + p.G, *mn = rs + p.G, *mm = mn + GN_CT, *m2 = mm + GN_CT;
   const int tid = threadIdx.x, n = blockIdx.y, chunk = p.chunks - 1 - blockIdx.x;
-  // J threads per group merge strided lists of chunks in order, then pairs
-  const int J = p.G >= GN_CT ? 1 : GN_CT / p.G;
-  for (int g0 = 0; g0 < p.G; g0 += GN_CT / J) {
-    const int j = tid / (GN_CT / J), g = g0 + tid - j * (GN_CT / J);
-    GnMom m = {0.f, 0.f, 0.f};
-    if (j < J && g < p.G && tid < J * (GN_CT / J))
-      for (int k = j; k < p.chunks; k += J) {
-        const float* o = p.part + 2 * (((long long)n * p.chunks + k) * p.G + g);
-        const int rows = min(p.rows, p.P - k * p.rows);
-        m = gn_merge(m, {(float)rows * (float)p.Cg, o[0], o[1]});
-      }
-    mn[tid] = m.n;
-    mm[tid] = m.mean;
-    m2[tid] = m.m2;
-    __syncthreads();
-    if (tid < GN_CT / J && g < p.G) {
-      for (int k = 1; k < J; ++k) {
-        const int i = tid + k * (GN_CT / J);
-        m = gn_merge(m, {mn[i], mm[i], m2[i]});
-      }
-      mu[g] = m.mean;
-      rs[g] = 1.f / sqrtf(m.m2 / m.n + p.eps);
-      if (blockIdx.x == 0) {
-        p.stats[2 * ((long long)n * p.G + g)] = mu[g];
-        p.stats[2 * ((long long)n * p.G + g) + 1] = rs[g];
-      }
-    }
-    __syncthreads();
-  }
   const int CV = p.C / V, RP = CV < GN_CT ? GN_CT / CV : 1;
   const int row0 = chunk * p.rows, row1 = min(row0 + p.rows, p.P);
   const int rr = CV < GN_CT ? tid / CV : 0;
@@ -473,8 +578,9 @@ __global__ __launch_bounds__(GN_CT) void gn_apply_kernel(const GnArgs p) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = cv * V + v, g = c / p.Cg;
-      mean[v] = mu[g];
-      ga[v] = rs[g] * (p.gamma ? p.gamma[c] : 1.f);
+      const float2 st = *reinterpret_cast<const float2*>(p.stats + 2 * ((long long)n * p.G + g));
+      mean[v] = st.x;
+      ga[v] = st.y * (p.gamma ? p.gamma[c] : 1.f);
       be[v] = p.beta ? p.beta[c] : 0.f;
     }
     const long long base = (long long)n * p.P * p.C + (long long)cv * V;
@@ -494,6 +600,7 @@ __global__ __launch_bounds__(GN_CT) void gn_apply_kernel(const GnArgs p) {
           for (int v = 0; v < V; ++v) f[v] = (f[v] - mean[v]) * ga[v] + be[v];
           gn_act<V>(f, p.act);
           *reinterpret_cast<Raw*>(y + (long long)(row + i * RP) * p.C) = gn_pack<T, V>(f);
+          gn_row_done();
         }
     }
   }
@@ -549,6 +656,7 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_sums_kernel(const GnArgs p) {
               a[v] += d[v];
               b[v] += d[v] * f[v];
             }
+            gn_row_done();
           }
       }
 #pragma unroll
@@ -586,9 +694,7 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_merge_kernel(const GnArgs p) {
     gn_sum_rows<GN_CT>(sa, W, J, tid);
     gn_sum_rows<GN_CT>(sb, W, J, tid);
     if (ok && j == 0) {
-      float* cs = p.csum + 2 * ((long long)n * p.C + c);
-      cs[0] = sa[w];
-      cs[1] = sb[w];
+      gn_channel_out(p, n, c, sa[w], sb[w]);
       const float ga = p.gamma ? p.gamma[c] : 1.f;
       ta += sa[w] * ga;
       tb += sb[w] * ga;
@@ -606,10 +712,30 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_merge_kernel(const GnArgs p) {
   }
 }
 
+// dgamma / dbeta of channel c from the samples' sums, in sample order
+__device__ __forceinline__ void gn_param_grad(const GnArgs& p, int c) {
+  if (c >= p.C) return;
+  float a = 0.f, b = 0.f;
+  for (int n = 0; n < p.N; ++n) {
+    const float2 s = *reinterpret_cast<const float2*>(p.csum + 2 * ((long long)n * p.C + c));
+    a += s.x;
+    b += s.y;
+  }
+  if (p.dbeta) p.dbeta[c] = a;
+  if (p.dgamma) p.dgamma[c] = b;
+}
+__global__ __launch_bounds__(256) void gn_param_grad_kernel(const GnArgs p) { gn_param_grad(p, blockIdx.x * 256 + threadIdx.x); }
+
+// dx of a chunk; the workgroups of sample 0 behind the last chunk form dgamma / dbeta
 template <typename T, int V>
 __global__ __launch_bounds__(GN_CT) void gn_bwd_apply_kernel(const GnArgs p) {
   using Raw = typename GnVec<T, V>::type;
-  const int tid = threadIdx.x, n = blockIdx.y, chunk = p.chunks - 1 - blockIdx.x;
+  const int tid = threadIdx.x, n = blockIdx.y;
+  if ((int)blockIdx.x >= p.chunks) {
+    if (n == 0) gn_param_grad(p, ((int)blockIdx.x - p.chunks) * GN_CT + tid);
+    return;
+  }
+  const int chunk = p.chunks - 1 - blockIdx.x;
   const int CV = p.C / V, RP = CV < GN_CT ? GN_CT / CV : 1;
   const int row0 = chunk * p.rows, row1 = min(row0 + p.rows, p.P);
   const int rr = CV < GN_CT ? tid / CV : 0;
@@ -653,23 +779,10 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_apply_kernel(const GnArgs p) {
 #pragma unroll
           for (int v = 0; v < V; ++v) d[v] = (d[v] * ga[v] - a[v] - f[v] * b[v]) * rstd[v];
           *reinterpret_cast<Raw*>(dx + (long long)(row + i * RP) * p.C) = gn_pack<T, V>(d);
+          gn_row_done();
         }
     }
   }
-}
-
-// dgamma / dbeta from the samples' channel sums, in sample order
-__global__ __launch_bounds__(256) void gn_param_grad_kernel(const GnArgs p) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= p.C) return;
-  float a = 0.f, b = 0.f;
-  for (int n = 0; n < p.N; ++n) {
-    const float2 s = *reinterpret_cast<const float2*>(p.csum + 2 * ((long long)n * p.C + c));
-    a += s.x;
-    b += s.y;
-  }
-  if (p.dbeta) p.dbeta[c] = a;
-  if (p.dgamma) p.dgamma[c] = b;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -694,14 +807,10 @@ static GnPlan gn_plan(int N, int P, int C, int G, int elem) {
     pl.slab = k;
     pl.R = pieces <= 4 ? 4 : pieces <= 8 ? 8 : 16;
   }
-  const int cv = C / pl.V, rp = cv < GN_CT ? GN_CT / cv : 1;
-  // chunks of at least two loads of GN_U rows per thread; about 1024 workgroups, at most 128 partial results per sample to merge
-  const int most = ceil_div(P, 2 * GN_U * rp);
-  int want = ceil_div(1024, N);
-  if (want > 128) want = 128;
-  if (want > most) want = most;
-  if (want < 1) want = 1;
-  pl.rows = ceil_div(P, want);
+  // chunks of whole loads (GN_U rows of every thread): as many loads each as leave about 2048 workgroups, eight to a CU
+  const int cv = C / pl.V, rp = cv < GN_CT ? GN_CT / cv : 1, unit = GN_U * rp;
+  const int loads = ceil_div(ceil_div(P, unit), ceil_div(2048, N));
+  pl.rows = loads * unit;
   pl.chunks = ceil_div(P, pl.rows);
   return pl;
 }
@@ -743,16 +852,17 @@ template <typename T, int V> static int gn_run(const GnArgs& a, const GnPlan& pl
     if (!backward) {
       TRACE_LDS_OPT_IN((gn_stats_kernel<T, V>), 2 * GN_MAX_C * 4 + 4096, "group_norm");
       gn_stats_kernel<T, V><<<grid, GN_CT, lds_s, st>>>(a);
-      TRACE_LDS_OPT_IN((gn_apply_kernel<T, V>), 4 * GN_MAX_C * 4 + 3 * GN_CT * 4, "group_norm");
-      gn_apply_kernel<T, V><<<grid, GN_CT, (2 * a.C + 2 * a.G + 3 * GN_CT) * 4, st>>>(a);
+      gn_merge_kernel<<<dim3(a.G, a.N), 64, 0, st>>>(a);
+      gn_apply_kernel<T, V><<<grid, GN_CT, 0, st>>>(a);
     } else {
       TRACE_LDS_OPT_IN((gn_bwd_sums_kernel<T, V>), 2 * GN_MAX_C * 4 + 4096, "group_norm backward");
       gn_bwd_sums_kernel<T, V><<<grid, GN_CT, lds_s, st>>>(a);
       gn_bwd_merge_kernel<<<dim3(a.G, a.N), GN_CT, 0, st>>>(a);
-      gn_bwd_apply_kernel<T, V><<<grid, GN_CT, 0, st>>>(a);
+      const int extra = a.N > 1 && (a.dgamma || a.dbeta) ? ceil_div(a.C, GN_CT) : 0;
+      gn_bwd_apply_kernel<T, V><<<dim3(pl.chunks + extra, a.N), GN_CT, 0, st>>>(a);
     }
   }
-  if (backward && (a.dgamma || a.dbeta)) gn_param_grad_kernel<<<ceil_div(a.C, 256), 256, 0, st>>>(a);
+  if (backward && pl.slab && a.N > 1 && (a.dgamma || a.dbeta)) gn_param_grad_kernel<<<ceil_div(a.C, 256), 256, 0, st>>>(a);
   return check_launch(backward ? "group_norm backward" : "group_norm");
 }
 
@@ -795,6 +905,10 @@ static int gn_call(bool backward, const T* x, const T* dy, int N, long long P, i
   a.gsum = reinterpret_cast<float*>(w + csum);
   a.part = reinterpret_cast<float*>(w + csum + gsum);
   a.slab = pl.slab;
+  if (pl.slab) {
+    const int sw = pl.slab * a.Cg / pl.V, cvg = a.Cg % pl.V ? 0 : a.Cg / pl.V;
+    a.pow2 = cvg && (sw & (sw - 1)) == 0 && (cvg & (cvg - 1)) == 0;
+  }
   a.rows = pl.rows;
   a.chunks = pl.chunks;
   if constexpr (std::is_same<T, float>::value) {

@@ -9,7 +9,7 @@ Launch plans: the I3D backbone is ~130 launches of fixed shape per batch.  `reco
 launch (same role as a HIP graph, but launch-by-launch so the per-launch event trace still works).
 """
 import ctypes
-
+import functools
 import os
 
 import torch
@@ -936,24 +936,51 @@ def pair_assemble(det_labels, det_scores, X, Y, low_s, low_o, part_s, part_o, fr
     return sl, ol, ss, os_, so_bias, so_part
 
 
+# ------------------------------------------------------------------ operators of a training step
+def _p(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _call(name, fn, dev, *args):
+    """One C-ABI call on the current stream of the operands' device, whichever device is current."""
+    if dev.index == torch._C._cuda_getDevice():
+        rc = fn(*args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev.index))
+    if rc != 0:
+        L.check(rc, name)
+
+
+def _scratch(nbytes, dev):
+    """Scratch of one call.  Its own allocation, not the shared split-K buffer: calls on several streams and captured
+    graphs then never share it (the allocator orders its reuse on the stream, a graph keeps its own)."""
+    return torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
+
+
 def _attn_operand(t, name):
     """(B, N, heads, D) bf16 on the GPU as the kernels take it: last dimension contiguous, rows 16-byte aligned, the other
     strides multiples of 8 elements (any order, 0 where a dimension is broadcast).  Other layouts are copied."""
-    L.require_gpu(t)
+    if not t.is_cuda:
+        L.require_gpu(t)
     if t.dtype != torch.bfloat16:
         raise RuntimeError("attention: %s must be bfloat16 (got %s)" % (name, t.dtype))
     if t.dim() != 4:
         raise RuntimeError("attention: %s must be (batch, rows, heads, head_dim), got %d dimensions" % (name, t.dim()))
-    if t.numel() and ((t.shape[3] > 1 and t.stride(3) != 1) or any(s % 8 for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1) or t.data_ptr() % 16):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
+    if not (t.is_contiguous() and t.shape[3] % 8 == 0 and t.data_ptr() % 16 == 0) and t.numel():
+        sb, sn, sh, sd = (s if n > 1 else 0 for s, n in zip(t.stride(), t.shape))
+        if sd > 1 or (sb | sn | sh) % 8 or sn >= 1 << 24 or t.data_ptr() % 16 or (sd == 0 and t.shape[3] > 1):
+            t = t.contiguous()
+            if t.data_ptr() % 16:
+                t = t.clone()
     return t
 
 
 def _attn_strides(t):
     # a dimension of one element may carry any stride: it is never stepped over
-    return (L.c_longlong * 3)(*[s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])])
+    b, n, h, _ = t.shape
+    s = t.stride()
+    return (s[0] if b > 1 else 0, s[1] if n > 1 else 0, s[2] if h > 1 else 0)
 
 
 def _attn_len(t, name, B, dev):
@@ -978,67 +1005,57 @@ def _attn_desc(q, k, v, scale, causal, q_len, kv_len):
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise RuntimeError("attention: scale must be positive and finite (got %r)" % scale)
-    d = L.AttentionDesc()
-    d.batch, d.q_rows, d.k_rows, d.heads, d.kv_heads, d.head_dim = B, Nq, k.shape[1], H, Hk, D
-    d.causal, d.scale = int(bool(causal)), scale
-    d.stride_q, d.stride_k, d.stride_v = _attn_strides(q), _attn_strides(k), _attn_strides(v)
-    d.q_len = None if q_len is None else q_len.data_ptr()
-    d.kv_len = None if kv_len is None else kv_len.data_ptr()
-    return d
+    return L.AttentionDesc(B, Nq, k.shape[1], H, Hk, D, 1 if causal else 0, scale, _attn_strides(q), _attn_strides(k),
+                           _attn_strides(v), (0, 0, 0), _p(q_len), _p(kv_len))
 
 
-def _scratch(nbytes, dev):
-    """Scratch of one call.  Its own allocation, not the shared split-K buffer: calls on several streams and captured
-    graphs then never share it (the allocator orders its reuse on the stream, a graph keeps its own)."""
-    return torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
-
-
-def attention(q, k, v, scale=None, causal=False, q_len=None, kv_len=None, return_lse=False):
-    """Softmax attention: q (B,Nq,H,D), k / v (B,Nk,Hkv,D) bf16 -> (B,Nq,H,D) bf16; with return_lse also log-sum-exp
-    (B,H,Nq) f32 (what `attention_backward` takes).  H is a multiple of Hkv: query head h reads key head h // (H / Hkv).
-    scale: None = D ** -0.5.  q_len / kv_len: int32 (B) on the device, rows of each batch entry that count (None: all;
-    values are clamped to 0 .. N); causal: query i sees key j <= i + kv_len - q_len.  A row behind q_len or without a key to see is
-    zero, with lse = -inf; rows behind a length are never read.  D % 8 == 0, 8 .. 512; the operands' rows may be strided
-    (views of a packed projection are taken as they are, other layouts are copied).  Keys and values in front of kv_len
-    must be finite, also those that `causal` hides from some rows."""
+def attention(q, k, v, scale=None, causal=False, q_len=None, kv_len=None, return_lse=False, for_backward=False):
+    """Softmax attention: q (B,Nq,H,D), k / v (B,Nk,Hkv,D) bf16 -> (B,Nq,H,D) bf16.  H is a multiple of Hkv: query head h
+    reads key head h // (H / Hkv).  scale: None = D ** -0.5.  q_len / kv_len: int32 (B) on the device, rows of each batch entry
+    that count (None: all; values are clamped to 0 .. N); causal: query i sees key j <= i + kv_len - q_len.  A row behind q_len
+    or without a key to see is zero; rows behind a length are never read.  D % 8 == 0, 8 .. 512; the operands' rows may be
+    strided (views of a packed projection are taken as they are, other layouts are copied).  Keys and values in front of
+    kv_len must be finite, also those that `causal` hides from some rows.
+    return_lse: -> (out, lse), lse (B,H,Nq) f32 the log-sum-exp of each row's scaled scores, -inf where it sees no key.
+    for_backward: -> (out, lse, rest), what `attention_backward` takes; rest is a second tensor like out, what rounding lost."""
     q, k, v = _attn_operand(q, "q"), _attn_operand(k, "k"), _attn_operand(v, "v")
     B, Nq, H, D = q.shape
-    q_len, kv_len = _attn_len(q_len, "q_len", B, q.device), _attn_len(kv_len, "kv_len", B, q.device)
+    dev = q.device
+    q_len, kv_len = _attn_len(q_len, "q_len", B, dev), _attn_len(kv_len, "kv_len", B, dev)
     d = _attn_desc(q, k, v, scale, causal, q_len, kv_len)
-    out = torch.empty((B, Nq, H, D), dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty((B, H, Nq), dtype=torch.float32, device=q.device) if return_lse else None
+    out = torch.empty((B, Nq, H, D), dtype=torch.bfloat16, device=dev)
+    lse = torch.empty((B, H, Nq), dtype=torch.float32, device=dev) if return_lse or for_backward else None
+    rest = torch.empty_like(out) if for_backward else None
     lib = L.lib()
-    with torch.cuda.device(q.device):
-        n = lib.trace_attention_fwd_workspace_bytes(d)
-        ws = _scratch(n, q.device)
-        L.check(lib.trace_attention_fwd_bf16(d, L.ptr(q), L.ptr(k), L.ptr(v), L.ptr(out), L.ptr(lse), L.ptr(ws), n, L.stream()),
-                "attention")
-    return (out, lse) if return_lse else out
+    n = lib.trace_attention_fwd_workspace_bytes(d)
+    ws = _scratch(n, dev)
+    _call("attention", lib.trace_attention_fwd_bf16, dev, d, _p(q), _p(k), _p(v), _p(out), _p(lse), _p(rest), _p(ws), n)
+    return (out, lse, rest) if for_backward else (out, lse) if return_lse else out
 
 
-def attention_backward(dout, q, k, v, out, lse, scale=None, causal=False, q_len=None, kv_len=None):
-    """(dq, dk, dv) bf16 of `attention` for the output gradient dout (B,Nq,H,D) bf16; out / lse as `attention(...,
-    return_lse=True)` returned them for the same operands and settings.  The probabilities are recomputed from lse; the
+def attention_backward(dout, q, k, v, out, lse, rest, scale=None, causal=False, q_len=None, kv_len=None):
+    """(dq, dk, dv) bf16 of `attention` for the output gradient dout (B,Nq,H,D) bf16; out / lse / rest as `attention(...,
+    for_backward=True)` returned them for the same operands and settings.  The probabilities are recomputed from lse; the
     gradients of a key head that several query heads share are summed in f32, in a fixed order."""
     q, k, v, dout = (_attn_operand(t, n) for t, n in ((q, "q"), (k, "k"), (v, "v"), (dout, "dout")))
     B, Nq, H, D = q.shape
-    q_len, kv_len = _attn_len(q_len, "q_len", B, q.device), _attn_len(kv_len, "kv_len", B, q.device)
+    dev = q.device
+    q_len, kv_len = _attn_len(q_len, "q_len", B, dev), _attn_len(kv_len, "kv_len", B, dev)
     d = _attn_desc(q, k, v, scale, causal, q_len, kv_len)
-    out = _bf16(out, "attention: out")
-    if lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (B, H, Nq) or lse.device != q.device:
+    if lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (B, H, Nq) or lse.device != dev:
         raise RuntimeError("attention_backward: lse must be the (batch, heads, rows) float32 tensor of the forward call")
-    if out.shape != q.shape or dout.shape != q.shape or out.device != q.device or dout.device != q.device:
-        raise RuntimeError("attention_backward: out %s / dout %s do not match q %s" % (tuple(out.shape), tuple(dout.shape), tuple(q.shape)))
+    for t, n in ((out, "out"), (rest, "rest"), (dout, "dout")):
+        if t.shape != q.shape or t.device != dev or t.dtype != torch.bfloat16 or not (t.is_contiguous() or t is dout):
+            raise RuntimeError("attention_backward: %s %s %s does not match q %s" % (n, tuple(t.shape), t.dtype, tuple(q.shape)))
     d.stride_do = _attn_strides(dout)
-    dq = torch.empty((B, Nq, H, D), dtype=torch.bfloat16, device=q.device)
-    dk = torch.empty(tuple(k.shape), dtype=torch.bfloat16, device=q.device)
-    dv = torch.empty(tuple(k.shape), dtype=torch.bfloat16, device=q.device)
+    dq = torch.empty((B, Nq, H, D), dtype=torch.bfloat16, device=dev)
+    dkv = torch.empty((2,) + tuple(k.shape), dtype=torch.bfloat16, device=dev)
+    dk, dv = dkv.unbind(0)
     lib = L.lib()
-    with torch.cuda.device(q.device):
-        n = lib.trace_attention_bwd_workspace_bytes(d)
-        ws = _scratch(n, q.device)
-        L.check(lib.trace_attention_bwd_bf16(d, L.ptr(q), L.ptr(k), L.ptr(v), L.ptr(out), L.ptr(lse), L.ptr(dout), L.ptr(dq),
-                                             L.ptr(dk), L.ptr(dv), L.ptr(ws), n, L.stream()), "attention_backward")
+    n = lib.trace_attention_bwd_workspace_bytes(d)
+    ws = _scratch(n, dev)
+    _call("attention_backward", lib.trace_attention_bwd_bf16, dev, d, _p(q), _p(k), _p(v), _p(out), _p(lse), _p(rest), _p(dout),
+          _p(dq), _p(dk), _p(dv), _p(ws), n)
     return dq, dk, dv
 
 
@@ -1048,7 +1065,8 @@ _GN_ACT = dict(_ACT, silu=EPI_SILU)
 
 def _map(t, name):
     """bf16 or f32, contiguous, 16-byte aligned (copied where it is not)."""
-    L.require_gpu(t)
+    if not t.is_cuda:
+        L.require_gpu(t)
     if t.dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError("%s must be bfloat16 or float32 (got %s)" % (name, t.dtype))
     t = t.contiguous()
@@ -1060,21 +1078,23 @@ def _gn_args(x, groups, gamma, beta, act, what):
         raise RuntimeError("%s: act %r (None, 'relu', 'leaky' or 'silu')" % (what, act))
     if x.dim() < 2:
         raise RuntimeError("%s: x must be (N, ..., C)" % what)
-    N, C = x.shape[0], x.shape[-1]
+    shape = x.shape
+    N, C = shape[0], shape[-1]
     P = 1
-    for s in x.shape[1:-1]:
+    for s in shape[1:-1]:
         P *= s
     groups = int(groups)
     if groups < 1 or C < 1 or C % groups:
         raise RuntimeError("%s: %d channels in %d groups" % (what, C, groups))
-    par = []
     for t, n in ((gamma, "gamma"), (beta, "beta")):
-        if t is not None:
-            if t.device != x.device or tuple(t.shape) != (C,):
-                raise RuntimeError("%s: %s must hold one value per channel on x's device" % (what, n))
-            t = _f32(t, n)
-        par.append(t)
-    return N, P, C, groups, par[0], par[1]
+        if t is not None and (t.device != x.device or t.dim() != 1 or t.shape[0] != C):
+            raise RuntimeError("%s: %s must hold one value per channel on x's device" % (what, n))
+    return N, P, C, groups, None if gamma is None else _f32(gamma, "gamma"), None if beta is None else _f32(beta, "beta")
+
+
+@functools.lru_cache(maxsize=1024)
+def _gn_workspace(N, P, C, G, backward):
+    return L.lib().trace_group_norm_workspace_bytes(N, P, C, G, backward)
 
 
 def group_norm_act(x, groups, gamma=None, beta=None, eps=1e-5, act=None, return_stats=False):
@@ -1084,17 +1104,16 @@ def group_norm_act(x, groups, gamma=None, beta=None, eps=1e-5, act=None, return_
     `group_norm_act_backward` takes."""
     x = _map(x, "group_norm_act: x")
     N, P, C, groups, gamma, beta = _gn_args(x, groups, gamma, beta, act, "group_norm_act")
-    if not float(eps) >= 0.0:
+    if not eps >= 0.0:
         raise RuntimeError("group_norm_act: eps must not be negative")
+    dev = x.device
     y = torch.empty_like(x)
-    stats = torch.empty((N, groups, 2), dtype=torch.float32, device=x.device)
+    stats = torch.empty((N, groups, 2), dtype=torch.float32, device=dev)
     lib = L.lib()
-    fn = lib.trace_group_norm_act_bf16 if x.dtype == torch.bfloat16 else lib.trace_group_norm_act_f32
-    with torch.cuda.device(x.device):
-        n = lib.trace_group_norm_workspace_bytes(N, P, C, groups, 0)
-        ws = _scratch(n, x.device)
-        L.check(fn(L.ptr(x), N, P, C, groups, L.ptr(gamma), L.ptr(beta), float(eps), _GN_ACT[act], L.ptr(y), L.ptr(stats),
-                   L.ptr(ws), n, L.stream()), "group_norm_act")
+    n = _gn_workspace(N, P, C, groups, 0)
+    ws = _scratch(n, dev)
+    _call("group_norm_act", lib.trace_group_norm_act_bf16 if x.dtype == torch.bfloat16 else lib.trace_group_norm_act_f32, dev,
+          _p(x), N, P, C, groups, _p(gamma), _p(beta), eps, _GN_ACT[act], _p(y), _p(stats), _p(ws), n)
     return (y, stats) if return_stats else y
 
 
@@ -1103,20 +1122,19 @@ def group_norm_act_backward(dy, x, stats, groups, gamma=None, beta=None, act=Non
     dgamma / dbeta (C) f32, None without param_grads."""
     x, dy = _map(x, "group_norm_act_backward: x"), _map(dy, "group_norm_act_backward: dy")
     N, P, C, groups, gamma, beta = _gn_args(x, groups, gamma, beta, act, "group_norm_act_backward")
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+    dev = x.device
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != dev:
         raise RuntimeError("group_norm_act_backward: dy %s %s for x %s %s" % (tuple(dy.shape), dy.dtype, tuple(x.shape), x.dtype))
-    if stats.device != x.device or stats.dtype != torch.float32 or tuple(stats.shape) != (N, groups, 2) or not stats.is_contiguous():
+    if stats.device != dev or stats.dtype != torch.float32 or stats.shape != (N, groups, 2) or not stats.is_contiguous():
         raise RuntimeError("group_norm_act_backward: stats must be the (N, groups, 2) float32 tensor of the forward call")
     dx = torch.empty_like(x)
-    dg = torch.empty((2, C), dtype=torch.float32, device=x.device) if param_grads else (None, None)
+    dg, db = torch.empty((2, C), dtype=torch.float32, device=dev).unbind(0) if param_grads else (None, None)
     lib = L.lib()
-    fn = lib.trace_group_norm_act_bwd_bf16 if x.dtype == torch.bfloat16 else lib.trace_group_norm_act_bwd_f32
-    with torch.cuda.device(x.device):
-        n = lib.trace_group_norm_workspace_bytes(N, P, C, groups, 1)
-        ws = _scratch(n, x.device)
-        L.check(fn(L.ptr(x), L.ptr(dy), N, P, C, groups, L.ptr(gamma), L.ptr(beta), L.ptr(stats), _GN_ACT[act], L.ptr(dx),
-                   L.ptr(dg[0]), L.ptr(dg[1]), L.ptr(ws), n, L.stream()), "group_norm_act_backward")
-    return dx, dg[0], dg[1]
+    n = _gn_workspace(N, P, C, groups, 1)
+    ws = _scratch(n, dev)
+    _call("group_norm_act_backward", lib.trace_group_norm_act_bwd_bf16 if x.dtype == torch.bfloat16 else lib.trace_group_norm_act_bwd_f32,
+          dev, _p(x), _p(dy), N, P, C, groups, _p(gamma), _p(beta), _p(stats), _GN_ACT[act], _p(dx), _p(dg), _p(db), _p(ws), n)
+    return dx, dg, db
 
 
 def _drop_args(p, seed, offset, step, act, dev, what):
@@ -1143,26 +1161,24 @@ def dropout_act(x, p, seed, offset=0, act=None, step=None):
     thr, seed, offset = _drop_args(p, seed, offset, step, act, x.device, "dropout_act")
     y = torch.empty_like(x)
     lib = L.lib()
-    fn = lib.trace_dropout_act_bf16 if x.dtype == torch.bfloat16 else lib.trace_dropout_act_f32
-    with torch.cuda.device(x.device):
-        L.check(fn(L.ptr(x), x.numel(), thr, seed, offset, L.ptr(step), _ACT[act], L.ptr(y), L.stream()), "dropout_act")
+    _call("dropout_act", lib.trace_dropout_act_bf16 if x.dtype == torch.bfloat16 else lib.trace_dropout_act_f32, x.device,
+          _p(x), x.numel(), thr, seed, offset, _p(step), _ACT[act], _p(y))
     return y
 
 
 def dropout_act_backward(dy, x, p, seed, offset=0, act=None, step=None):
     """dx of `dropout_act`: the mask is drawn again from the same (seed, offset, step).  x may be None without an activation."""
     dy = _map(dy, "dropout_act_backward: dy")
-    thr, seed, offset = _drop_args(p, seed, offset, step, act, dy.device, "dropout_act_backward")
+    dev = dy.device
+    thr, seed, offset = _drop_args(p, seed, offset, step, act, dev, "dropout_act_backward")
     if _ACT[act]:
-        if x is None or x.shape != dy.shape or x.dtype != dy.dtype or x.device != dy.device:
+        if x is None or x.shape != dy.shape or x.dtype != dy.dtype or x.device != dev:
             raise RuntimeError("dropout_act_backward: x must match dy where an activation follows")
         x = _map(x, "dropout_act_backward: x")
     else:
         x = None
     dx = torch.empty_like(dy)
     lib = L.lib()
-    fn = lib.trace_dropout_act_bwd_bf16 if dy.dtype == torch.bfloat16 else lib.trace_dropout_act_bwd_f32
-    with torch.cuda.device(dy.device):
-        L.check(fn(L.ptr(x), L.ptr(dy), dy.numel(), thr, seed, offset, L.ptr(step), _ACT[act], L.ptr(dx), L.stream()),
-                "dropout_act_backward")
+    _call("dropout_act_backward", lib.trace_dropout_act_bwd_bf16 if dy.dtype == torch.bfloat16 else lib.trace_dropout_act_bwd_f32,
+          dev, _p(x), _p(dy), dy.numel(), thr, seed, offset, _p(step), _ACT[act], _p(dx))
     return dx
