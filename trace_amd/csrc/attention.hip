@@ -56,40 +56,46 @@ template <int D> __device__ __forceinline__ int at_key(int r) {
 }
 template <int D> __device__ __forceinline__ int at_off(int r, int chunk) { return r * (2 * D) + ((chunk ^ at_key<D>(r)) << 4); }
 
-// One wave's share of the LDS-DMA of a ROWS x D tile (whole workgroup: NW waves).
+// One wave's share of the LDS-DMA of a ROWS x D tile (whole workgroup: NW waves).  Consecutive loads of a wave are STEP rows
+// apart; where that is a multiple of eight rows the key repeats, and one lane offset serves them all.
 template <int D, int ROWS, int NW> struct AtLoader {
   static constexpr int CPR = D / 8;
   static constexpr int INST = ROWS * CPR / 64, N = INST < NW ? 1 : INST / NW;   // loads of 1 KiB: in all, per wave
+  static constexpr int STEP = 64 * NW / CPR, M = STEP % 8 == 0 ? 1 : N;
   static_assert(ROWS * CPR % 64 == 0 && (INST < NW || INST % NW == 0), "whole instructions per wave");
-  uint32_t off[N];   // bytes from the tile's first row (rows x stride stay below 2^31: at_check)
+  uint32_t off[M];   // bytes from the tile's first row (rows x stride stay below 2^31: at_check)
   unsigned colok;    // bit j: this lane's chunk of load j lies inside head_dim
   __device__ __forceinline__ void init(long long row_stride, int d, int wave, int lane) {
     colok = 0;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
+    for (int j = 0; j < M; ++j) {
       const int id = (j * NW + wave) * 64 + lane, row = id / CPR, c = (id % CPR) ^ at_key<D>(row);
       off[j] = (uint32_t)(row * row_stride * 2 + c * 16);
       if (c * 8 < d) colok |= 1u << j;
     }
   }
   // `rows` rows from `base` (uniform); further rows and the columns behind head_dim (`d` of D) read zeros
-  __device__ __forceinline__ void issue(char* lds, const uint16_t* base, int rows, int d, int wave, int lane) const {
+  __device__ __forceinline__ void issue(char* lds, const uint16_t* base, long long row_stride, int rows, int d, int wave, int lane) const {
     if (INST < NW && wave >= INST) return;
     const char* b = reinterpret_cast<const char*>(base);
+    const long long step = M == 1 ? STEP * row_stride * 2 : 0;
     if (rows >= ROWS && d == D) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) glds16(b + off[j], lds + (j * NW + wave) * 1024);
+      for (int j = 0; j < N; ++j) glds16(b + j * step + off[M == 1 ? 0 : j], lds + (j * NW + wave) * 1024);
       return;
     }
     const char* zero = reinterpret_cast<const char*>(g_at_zero);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int row = ((j * NW + wave) * 64 + lane) / CPR;
-      const bool ok = ((colok >> j) & 1u) && row < rows;
-      glds16(ok ? b + off[j] : zero, lds + (j * NW + wave) * 1024);
+      const bool ok = ((colok >> (M == 1 ? 0 : j)) & 1u) && row < rows;
+      glds16(ok ? b + j * step + off[M == 1 ? 0 : j] : zero, lds + (j * NW + wave) * 1024);
     }
   }
 };
+
+// in a branch that every lane of the wave takes or none: keeps the compiler from running it always, with the results selected
+__device__ __forceinline__ void at_keep_branch() { asm volatile(""); }
 
 // B operand: a row of an operand as column of the product, 8 columns from 32 (kc0 + kc) + 8 g, straight from memory
 template <int KC> __device__ __forceinline__ void at_load_cols(at_s8 (&f)[KC], const uint16_t* row, bool ok, int kc0, int d, int g) {
@@ -111,11 +117,13 @@ __device__ __forceinline__ at_s8 at_pack8(const at_f4& a, const at_f4& b) {
 
 // bf16 of what at_pack8 lost
 __device__ __forceinline__ at_s8 at_lost8(const at_f4& a, const at_f4& b, const at_s8& packed) {
+  union { at_s8 v; uint32_t u[4]; } w;
+  w.v = packed;
   at_f4 x, y;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    x[r] = a[r] - bf16_to_f32((uint16_t)packed[r]);
-    y[r] = b[r] - bf16_to_f32((uint16_t)packed[4 + r]);
+    x[r] = a[r] - __uint_as_float(r & 1 ? w.u[r >> 1] & 0xffff0000u : w.u[r >> 1] << 16);
+    y[r] = b[r] - __uint_as_float(r & 1 ? w.u[2 + (r >> 1)] & 0xffff0000u : w.u[2 + (r >> 1)] << 16);
   }
   return at_pack8(x, y);
 }
@@ -271,8 +279,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
   const uint16_t* vb = p.v + b * p.sv[0] + hk * p.sv[2];
   auto issue = [&](int t) {
     const int st = ((t - t0) & 1) * (2 * TILE), k0 = t * BN;
-    lk.issue(smem + st, kb + k0 * p.sk[1], kend - k0, p.D, wave, lane);
-    lv.issue(smem + st + TILE, vb + k0 * p.sv[1], kend - k0, p.D, wave, lane);
+    lk.issue(smem + st, kb + k0 * p.sk[1], p.sk[1], kend - k0, p.D, wave, lane);
+    lv.issue(smem + st + TILE, vb + k0 * p.sv[1], p.sv[1], kend - k0, p.D, wave, lane);
   };
   const int row_at = at_row_base<D>(lane) ^ (wd * KC << 6), tr_at = (at_tr_base<D>(lane) ^ (wd * DT << 5)) + TILE;
 
@@ -301,6 +309,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
     at_score<D>(smem, row_at + stage, qf, s);
     if constexpr (DW > 1) at_exchange<ST, NT, DW>(smem + 4 * TILE, wave, lane, s);
     if (key0 + BN > wmin) {
+      at_keep_branch();
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -500,8 +509,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
   const uint16_t* vb = p.v + b * p.sv[0] + hk * p.sv[2];
   auto issue = [&](int t) {
     const int st = ((t - t0) & 1) * (2 * TILE), k0 = t * BN;
-    lk.issue(smem + st, kb + k0 * p.sk[1], kend - k0, p.D, wave, lane);
-    lv.issue(smem + st + TILE, vb + k0 * p.sv[1], kend - k0, p.D, wave, lane);
+    lk.issue(smem + st, kb + k0 * p.sk[1], p.sk[1], kend - k0, p.D, wave, lane);
+    lv.issue(smem + st + TILE, vb + k0 * p.sv[1], p.sv[1], kend - k0, p.D, wave, lane);
   };
   const int row_at = at_row_base<D>(lane) ^ (wd * KC << 6), tr_at = at_tr_base<D>(lane) ^ (wd * DT << 5);
   const float c = p.scale * AT_LOG2E;
@@ -540,13 +549,20 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float pr = __builtin_amdgcn_exp2f(s[st][nt][r] * c - lse2[nt]);
-          if (mask && key0 + st * 16 + 4 * g + r >= lim[nt]) pr = 0.f;
-          s[st][nt][r] = pr * dp[st][nt][r];
-        }
-      ds[nt] = at_pack8(s[0][nt], s[1][nt]);
+        for (int r = 0; r < 4; ++r) s[st][nt][r] = __builtin_amdgcn_exp2f(s[st][nt][r] * c - lse2[nt]);
     }
+    if (mask) {
+      at_keep_branch();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (key0 + st * 16 + 4 * g + r >= lim[nt]) s[st][nt][r] = 0.f;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) ds[nt] = at_pack8(s[0][nt] * dp[0][nt], s[1][nt] * dp[1][nt]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const at_s8 a = at_tr<D>(smem, (tr_at + stage) ^ (dt << 5));
@@ -577,13 +593,15 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
 // 32-row tiles of q and dout of every query head that reads it, so the gradients of shared heads are summed in a fixed order.
 // ---------------------------------------------------------------------------------------------------------------
 template <int D, int NT, int NW, int DW>
-__global__ __launch_bounds__(64 * NW, D >= 512 ? 1 : 2) void attn_bwd_kv_kernel(const AttnArgs p) {
+__global__ __launch_bounds__(64 * NW, 2) void attn_bwd_kv_kernel(const AttnArgs p) {
   constexpr int BQ = 32, TK = NW / DW * NT * 16, KC = D / 32 / DW, DT = D / 16 / DW;
   constexpr int TILE = BQ * D * 2;
-  extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of [q][dout], two of [32 lse, 32 -delta], exchange
+  constexpr bool VL = DW == 1;   // the values as a tile in LDS instead of registers, which the sums need
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of [q][dout], [v], two of [32 lse, 32 -delta], exchange
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wd = wave % DW, wr = wave / DW;
-  char* stats = smem + 4 * TILE;
+  constexpr int V_AT = 4 * TILE;
+  char* stats = smem + V_AT + (VL ? TK * D * 2 : 0);
   char* xbuf = stats + 512;
   const int u = at_unit(blockIdx.x, gridDim.x);
   const int tile = u % p.tiles, hk = (u / p.tiles) % p.Hk, b = u / p.tiles / p.Hk;
@@ -592,14 +610,14 @@ __global__ __launch_bounds__(64 * NW, D >= 512 ? 1 : 2) void attn_bwd_kv_kernel(
   const int key_first = tile * TK, wkey = key_first + wr * NT * 16;
 
   int key[NT];
-  at_s8 kf[NT][KC], vf[NT][KC];
+  at_s8 kf[NT][KC], vf[VL ? 1 : NT][KC];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     key[nt] = wkey + nt * 16 + (lane & 15);
     const bool ok = key[nt] < kvlen;
     const int kk = ok ? key[nt] : 0;
     at_load_cols<KC>(kf[nt], p.k + b * p.sk[0] + kk * p.sk[1] + hk * p.sk[2], ok, wd * KC, p.D, g);
-    at_load_cols<KC>(vf[nt], p.v + b * p.sv[0] + kk * p.sv[1] + hk * p.sv[2], ok, wd * KC, p.D, g);
+    if constexpr (!VL) at_load_cols<KC>(vf[nt], p.v + b * p.sv[0] + kk * p.sv[1] + hk * p.sv[2], ok, wd * KC, p.D, g);
   }
   at_f4 ak[DT][NT], av[DT][NT];
 #pragma unroll
@@ -623,8 +641,8 @@ __global__ __launch_bounds__(64 * NW, D >= 512 ? 1 : 2) void attn_bwd_kv_kernel(
   int head = 0, qt = 0;          // of the tile issued last
   auto issue = [&](int it) {
     const int par = (it - it0) & 1, q0 = qt * BQ;
-    lq.issue(smem + par * (2 * TILE), qb + head * p.sq[2] + q0 * p.sq[1], qlen - q0, p.D, wave, lane);
-    ld.issue(smem + par * (2 * TILE) + TILE, db + head * p.sdo[2] + q0 * p.sdo[1], qlen - q0, p.D, wave, lane);
+    lq.issue(smem + par * (2 * TILE), qb + head * p.sq[2] + q0 * p.sq[1], p.sq[1], qlen - q0, p.D, wave, lane);
+    ld.issue(smem + par * (2 * TILE) + TILE, db + head * p.sdo[2] + q0 * p.sdo[1], p.sdo[1], qlen - q0, p.D, wave, lane);
     if (wave == 0) {
       const int i = q0 + (lane & 31);
       const float* src = i < qlen ? stat + (long long)head * p.Nq + i : reinterpret_cast<const float*>(g_at_zero);
@@ -634,6 +652,11 @@ __global__ __launch_bounds__(64 * NW, D >= 512 ? 1 : 2) void attn_bwd_kv_kernel(
   const int row_at = at_row_base<D>(lane) ^ (wd * KC << 6), tr_at = at_tr_base<D>(lane) ^ (wd * DT << 5);
   const float c = p.scale * AT_LOG2E;
   if (it0 < it1) {
+    if constexpr (VL) {
+      AtLoader<D, TK, NW> lv;
+      lv.init(p.sv[1], p.D, wave, lane);
+      lv.issue(smem + V_AT, p.v + b * p.sv[0] + hk * p.sv[2] + key_first * p.sv[1], p.sv[1], kvlen - key_first, p.D, wave, lane);
+    }
     head = it0 / per_head;
     qt = qt0 + it0 - head * per_head;
     issue(it0);
@@ -650,10 +673,8 @@ __global__ __launch_bounds__(64 * NW, D >= 512 ? 1 : 2) void attn_bwd_kv_kernel(
     if (DW == 1 && p.causal && wkey > q0 + BQ - 1 + diff) continue;   // no key of this wave is seen
     at_f4 s[2][NT], dp[2][NT];
     const float* sp = reinterpret_cast<const float*>(stats + par * 256) + 4 * g;
-    at_f4 lse2[2];
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
-      lse2[st] = *reinterpret_cast<const at_f4*>(sp + st * 16) * AT_LOG2E;
       const at_f4 nd = *reinterpret_cast<const at_f4*>(sp + 32 + st * 16);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -662,12 +683,30 @@ __global__ __launch_bounds__(64 * NW, D >= 512 ? 1 : 2) void attn_bwd_kv_kernel(
       }
     }
     at_score<D>(smem, row_at + stage, kf, s);
-    at_score<D>(smem, row_at + stage + TILE, vf, dp);
+    if constexpr (VL) {
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc) {
+        at_s8 bv[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) bv[nt] = at_row(smem, V_AT + (row_at ^ (kc << 6)) + (wr * NT + nt) * 32 * D);
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const at_s8 a = at_row(smem, ((row_at + stage + TILE) ^ (kc << 6)) + st * 32 * D);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) dp[st][nt] = at_mfma(a, bv[nt], dp[st][nt]);
+        }
+      }
+    } else {
+      at_score<D>(smem, row_at + stage + TILE, vf, dp);
+    }
     if constexpr (DW > 1) {
       at_exchange<2, NT, DW>(xbuf, wave, lane, s);
       ring_barrier();
       at_exchange<2, NT, DW>(xbuf, wave, lane, dp);
     }
+    at_f4 lse2[2];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) lse2[st] = *reinterpret_cast<const at_f4*>(sp + st * 16) * AT_LOG2E;
     const bool mask = q0 + BQ > qlen || wkey + NT * 16 > kvlen || (p.causal && wkey + NT * 16 - 1 > q0 + diff);
     at_s8 pf[NT], ds[NT];
 #pragma unroll
@@ -675,15 +714,27 @@ __global__ __launch_bounds__(64 * NW, D >= 512 ? 1 : 2) void attn_bwd_kv_kernel(
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float pr = __builtin_amdgcn_exp2f(s[st][nt][r] * c - lse2[st][r]);
-          const int i = q0 + st * 16 + 4 * g + r;
-          if (mask && (i >= qlen || key[nt] >= kvlen || (p.causal && key[nt] > i + diff))) pr = 0.f;
-          s[st][nt][r] = pr;
-          dp[st][nt][r] *= pr;
-        }
+        for (int r = 0; r < 4; ++r) s[st][nt][r] = __builtin_amdgcn_exp2f(s[st][nt][r] * c - lse2[st][r]);
+    }
+    if (mask) {
+      at_keep_branch();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        // queries from `first` on see this key
+        const int first = key[nt] >= kvlen ? 0x7fffffff : p.causal ? key[nt] - diff : 0;
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = q0 + st * 16 + 4 * g + r;
+            if (i >= qlen || i < first) s[st][nt][r] = 0.f;
+          }
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
       pf[nt] = at_pack8(s[0][nt], s[1][nt]);
-      ds[nt] = at_pack8(dp[0][nt], dp[1][nt]);
+      ds[nt] = at_pack8(s[0][nt] * dp[0][nt], s[1][nt] * dp[1][nt]);
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
@@ -766,7 +817,7 @@ static AttnPlan at_plan(const trace_attention_desc* d) {
   pl.q_rows = bwd_rows;
   pl.q_tiles = ceil_div(d->q_rows, pl.q_rows);
   pl.q_splits = at_splits((long long)pl.q_tiles * d->heads * d->batch, ceil_div(d->k_rows, 32), 4, 2);
-  pl.k_rows = pl.D <= 256 ? 128 : 32;
+  pl.k_rows = pl.D <= 256 ? 128 : 64;
   pl.k_tiles = ceil_div(d->k_rows, pl.k_rows);
   pl.k_splits = at_splits((long long)pl.k_tiles * d->kv_heads * d->batch, ceil_div(d->q_rows, 32) * G, 4, waves);
   return pl;
@@ -833,7 +884,7 @@ template <int D, int NT, int NW, int DW> static int at_launch_q(const AttnArgs& 
   return 0;
 }
 template <int D, int NT, int NW, int DW> static int at_launch_kv(const AttnArgs& a, hipStream_t st) {
-  const int lds = 4 * 32 * D * 2 + 512 + (DW > 1 ? NW * 2 * NT * 1024 : 0);
+  const int lds = 4 * 32 * D * 2 + 512 + (DW > 1 ? NW * 2 * NT * 1024 : NW * NT * 16 * D * 2);
   TRACE_LDS_OPT_IN((attn_bwd_kv_kernel<D, NT, NW, DW>), lds, "attention backward");
   attn_bwd_kv_kernel<D, NT, NW, DW><<<dim3((unsigned)a.tiles * a.Hk * a.B, a.splits), 64 * NW, lds, st>>>(a);
   return 0;
@@ -979,8 +1030,8 @@ extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uin
       case 32: rc = at_launch_kv<32, 2, 4, 1>(a, st); break;
       case 64: rc = at_launch_kv<64, 2, 4, 1>(a, st); break;
       case 128: rc = at_launch_kv<128, 2, 4, 1>(a, st); break;
-      case 256: rc = at_launch_kv<256, 2, 8, 2>(a, st); break;
-      default: rc = at_launch_kv<512, 2, 4, 4>(a, st); break;
+      case 256: rc = at_launch_kv<256, 1, 8, 1>(a, st); break;
+      default: rc = at_launch_kv<512, 1, 8, 2>(a, st); break;
     }
     if (rc) return rc;
     if (int e = check_launch("attention backward (dk, dv)")) return e;
