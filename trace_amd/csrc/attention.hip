@@ -150,10 +150,28 @@ __device__ __forceinline__ at_f4 at_mfma(const at_s8& a, const at_s8& b, const a
 }
 
 // Workgroups go to the 8 XCDs round-robin and each XCD has its own L2: XCD x gets the x-th contiguous eighth of the
-// units, so the tiles that read one head's other operand share an L2.
-__device__ __forceinline__ int at_unit(int lin, int total) {
-  const int x = lin & 7, per = total >> 3, rem = total & 7;
-  return x * per + min(x, rem) + (lin >> 3);
+// (head, split, tile) units, so the tiles that read one head's other operand share an L2.  `uneven`: under a causal mask a
+// tile's work falls with its index (the caller counts from the longest); tile 0 of all heads and splits goes first then, so that
+// short ones fill the end: 2 x 4096 x 16 heads x 128, forward 211 -> 166 us, backward 566 -> 455 us.
+struct AtUnit {
+  int tile, split, head;   // head: of all batches
+};
+__device__ __forceinline__ AtUnit at_unit(int lin, int tiles, int splits, int heads, bool uneven) {
+  const int x = lin & 7, hs = heads * splits;
+  int t, h;
+  if (!uneven) {
+    const int total = tiles * hs, per = total >> 3, rem = total & 7, u = x * per + min(x, rem) + (lin >> 3);
+    t = u % tiles;
+    h = u / tiles;
+  } else if ((hs & 7) == 0) {   // neighbouring heads on one XCD
+    const int hx = hs >> 3, i = lin >> 3;
+    t = i / hx;
+    h = x * hx + i % hx;
+  } else {
+    t = lin / hs;
+    h = lin % hs;
+  }
+  return {t, h % splits, h / splits};
 }
 __device__ __forceinline__ int at_len(const int32_t* len, int b, int n) { return len ? min(max(len[b], 0), n) : n; }
 
@@ -175,19 +193,46 @@ template <bool FINE> __device__ __forceinline__ void at_store_out(const AttnArgs
               v[2] - bf16_to_f32((uint16_t)o.y), v[3] - bf16_to_f32((uint16_t)(o.y >> 16)));
 }
 
+// Fragments are read AT_AHEAD ahead of the products that take them: an LDS read takes longer than the NT products of one
+// fragment, and left alone hipcc reads each one right in front of its use.
+constexpr int AT_AHEAD = 4;
+__device__ __forceinline__ void at_order() { __builtin_amdgcn_sched_barrier(0); }
+
 // s[st][nt] (16-row tiles of a staged tile x 16 columns) += rows . columns over the wave's KC 32-column blocks
 template <int D, int ST, int NT, int KC>
 __device__ __forceinline__ void at_score(const char* smem, int at, const at_s8 (&f)[NT][KC], at_f4 (&s)[ST][NT]) {
+  constexpr int F = KC * ST, A = F < AT_AHEAD ? F : AT_AHEAD;
+  at_s8 a[A];
 #pragma unroll
-  for (int kc = 0; kc < KC; ++kc) {
+  for (int i = 0; i < A; ++i) a[i] = at_row(smem, (at ^ ((i / ST) << 6)) + (i % ST) * 32 * D);
 #pragma unroll
-    for (int st = 0; st < ST; ++st) {
-      const at_s8 a = at_row(smem, (at ^ (kc << 6)) + st * 32 * D);
+  for (int i = 0; i < F; ++i) {
+    const int kc = i / ST, st = i % ST, j = i + A;
+    const at_s8 x = a[i % A];
+    if (j < F) a[i % A] = at_row(smem, (at ^ ((j / ST) << 6)) + (j % ST) * 32 * D);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[st][nt] = at_mfma(a, f[nt][kc], s[st][nt]);
-    }
+    for (int nt = 0; nt < NT; ++nt) s[st][nt] = at_mfma(x, f[nt][kc], s[st][nt]);
+    at_order();
   }
 }
+
+// Transposed fragments of a tile in the order of a summing product: column blocks of 16, KK row blocks of 32 each
+template <int D, int DT, int KK> struct AtTrAhead {
+  static constexpr int F = DT * KK, A = F < AT_AHEAD ? F : AT_AHEAD;
+  at_s8 a[A];
+  __device__ __forceinline__ static at_s8 load(const char* smem, int at, int i) { return at_tr<D>(smem, (at ^ ((i / KK) << 5)) + (i % KK) * 64 * D); }
+  __device__ __forceinline__ void start(const char* smem, int at) {
+#pragma unroll
+    for (int i = 0; i < A; ++i) a[i] = load(smem, at, i);
+    at_order();
+  }
+  // fragment i, whose place the one A behind it takes
+  __device__ __forceinline__ at_s8 take(const char* smem, int at, int i) {
+    const at_s8 x = a[i % A];
+    if (i + A < F) a[i % A] = load(smem, at, i + A);
+    return x;
+  }
+};
 
 // DW waves of a row group hold partial scores over their share of head_dim: every one gets the sum, added in wave order
 // (equal bits in all of them).  Each wave's scores pass through its own part of the exchange buffer; the caller has a barrier
@@ -231,10 +276,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
   extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of [K tile][V tile], exchange buffer
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wd = wave % DW, wr = wave / DW;
-  const int u = at_unit(blockIdx.x, gridDim.x);
-  int tile = u % p.tiles;
-  const int unit = (u / p.tiles) % p.units, b = u / p.tiles / p.units;
-  if (p.causal) tile = p.tiles - 1 - tile;   // the longest rows first
+  const AtUnit u = at_unit(blockIdx.x, p.tiles, p.splits, p.units * p.B, p.causal);
+  const int tile = p.causal ? p.tiles - 1 - u.tile : u.tile;
+  const int unit = u.head % p.units, b = u.head / p.units;
   const int G = p.H / p.Hk, hk = unit * p.pack / G;
   const int qlen = at_len(p.q_len, b, p.Nq), kvlen = at_len(p.kv_len, b, p.Nk), diff = kvlen - qlen;
   const int nrows = p.pack * p.Nq;
@@ -270,7 +314,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
     if (last >= tile * TR) kend = p.causal ? min(max(last + diff + 1, 0), kvlen) : kvlen;
   }
   const int ntile = (kend + BN - 1) / BN, per = (ntile + p.splits - 1) / p.splits;
-  const int t0 = min((int)blockIdx.y * per, ntile), t1 = min(t0 + per, ntile);
+  const int t0 = min(u.split * per, ntile), t1 = min(t0 + per, ntile);
 
   AtLoader<D, BN, NW> lk, lv;
   lk.init(p.sk[1], p.D, wave, lane);
@@ -318,6 +362,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
           for (int r = 0; r < 4; ++r)
             if (key0 + st * 16 + 4 * g + r >= lim[nt]) s[st][nt][r] = -INFINITY;
     }
+    AtTrAhead<D, DT, BN / 32> va;
+    va.start(smem, tr_at + stage);
     at_s8 pf[BN / 32][NT], pl[BN / 32][NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -351,16 +397,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
       }
     }
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int i = 0; i < DT * (BN / 32); ++i) {
+      const int dt = i / (BN / 32), kk = i % (BN / 32);
+      const at_s8 a = va.take(smem, tr_at + stage, i);
 #pragma unroll
-      for (int kk = 0; kk < BN / 32; ++kk) {
-        const at_s8 a = at_tr<D>(smem, ((tr_at + stage) ^ (dt << 5)) + kk * 64 * D);
+      for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, pf[kk][nt], acc[dt][nt]);
+      if constexpr (FINE) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          acc[dt][nt] = at_mfma(a, pf[kk][nt], acc[dt][nt]);
-          if constexpr (FINE) acc[dt][nt] = at_mfma(a, pl[kk][nt], acc[dt][nt]);
-        }
+        for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, pl[kk][nt], acc[dt][nt]);
       }
+      at_order();
+    }
   }
   const bool split = p.splits > 1;
 #pragma unroll
@@ -372,7 +419,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
     const bool any = lim[nt] > 0 && sum > 0.f;
     const long long row = ((long long)b * p.H + row_h[nt]) * p.Nq + row_i[nt];
     if (split) {
-      const long long rows = (long long)p.B * p.H * p.Nq, at = blockIdx.y * rows + row;
+      const long long rows = (long long)p.B * p.H * p.Nq, at = u.split * rows + row;
       if (g == 0 && wd == 0) p.part_ml[at] = any ? make_float2(m[nt] * c, sum) : make_float2(-INFINITY, 0.f);
       if (!any) continue;
 #pragma unroll
@@ -393,32 +440,42 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
   }
 }
 
-// out / lse of a row from its splits' (max, sum, unnormalised out), in split order; one thread per four columns
+// out / lse of a row from its splits' (max, sum, unnormalised out).  A workgroup per row: a wave turns the splits' statistics
+// into weights (at most 64 splits), then groups of D / 4 threads add strided lists of splits, and the first group adds the groups.
 template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs p) {
-  const int dq = p.D >> 2;
-  const long long rows = (long long)p.B * p.H * p.Nq;
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= rows * dq) return;
-  const long long row = id / dq;
-  const int d = (int)(id - row * dq) * 4;
-  float mx = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, p.part_ml[s * rows + row].x);
-  float sum = 0.f;
-  at_f4 o = {0.f, 0.f, 0.f, 0.f};
-  if (mx != -INFINITY) {
-    for (int s = 0; s < p.splits; ++s) {
-      const float2 ml = p.part_ml[s * rows + row];
-      if (ml.y <= 0.f) continue;
-      const float w = __builtin_amdgcn_exp2f(ml.x - mx);
-      sum += w * ml.y;
-      o += w * *reinterpret_cast<const at_f4*>(p.part + (s * rows + row) * p.D + d);
-    }
+  __shared__ float weight[64];
+  __shared__ at_f4 red[256];
+  const int tid = threadIdx.x, lane = tid & 63, dq = p.D >> 2, groups = min(256 / dq, p.splits);
+  const long long rows = (long long)p.B * p.H * p.Nq, row = blockIdx.x;
+  if (tid < 64) {
+    const float2 ml = lane < p.splits ? p.part_ml[lane * rows + row] : make_float2(-INFINITY, 0.f);
+    float mx = ml.x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    const float w = ml.y > 0.f ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.f;
+    float sum = w * ml.y;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+    weight[lane] = sum > 0.f ? w / sum : 0.f;
+    if (lane == 0 && p.lse) p.lse[row] = sum > 0.f ? (mx + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  const int i = (int)(row % p.Nq), h = (int)(row / p.Nq % p.H);
-  const long long b = row / p.Nq / p.H;
-  at_store_out<FINE>(p, ((b * p.Nq + i) * p.H + h) * p.D + d, o * inv);
-  if (d == 0 && p.lse) p.lse[row] = sum > 0.f ? (mx + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
+  __syncthreads();
+  const int grp = tid / dq, d = (tid - grp * dq) * 4;
+  if (grp < groups) {
+    at_f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = grp; s < p.splits; s += groups)
+      if (weight[s] != 0.f) o += weight[s] * *reinterpret_cast<const at_f4*>(p.part + (s * rows + row) * p.D + d);   // else: never written
+    red[tid] = o;
+  }
+  __syncthreads();
+  if (grp == 0) {
+    at_f4 o = red[tid];
+    for (int k = 1; k < groups; ++k) o += red[k * dq + tid];
+    const int i = (int)(row % p.Nq), h = (int)(row / p.Nq % p.H);
+    const long long b = row / p.Nq / p.H;
+    at_store_out<FINE>(p, ((b * p.Nq + i) * p.H + h) * p.D + d, o);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -433,10 +490,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wd = wave % DW, wr = wave / DW;
   char* xbuf = smem + 4 * TILE;
-  const int u = at_unit(blockIdx.x, gridDim.x);
-  int tile = u % p.tiles;
-  const int h = (u / p.tiles) % p.H, b = u / p.tiles / p.H;
-  if (p.causal) tile = p.tiles - 1 - tile;
+  const AtUnit u = at_unit(blockIdx.x, p.tiles, p.splits, p.H * p.B, p.causal);
+  const int tile = p.causal ? p.tiles - 1 - u.tile : u.tile, h = u.head % p.H, b = u.head / p.H;
   const int hk = h / (p.H / p.Hk);
   const int qlen = at_len(p.q_len, b, p.Nq), kvlen = at_len(p.kv_len, b, p.Nk), diff = kvlen - qlen;
 
@@ -487,7 +542,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
-    if (row_i[nt] < qlen && g == 0 && wd == 0 && blockIdx.y == 0) p.ndelta[((long long)b * p.H + h) * p.Nq + row_i[nt]] = ndelta[nt];
+    if (row_i[nt] < qlen && g == 0 && wd == 0 && u.split == 0) p.ndelta[((long long)b * p.H + h) * p.Nq + row_i[nt]] = ndelta[nt];
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
     wmin = min(wmin, __shfl_xor(wmin, o));
@@ -500,7 +555,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
   const int last = min((tile + 1) * TR, qlen) - 1;
   if (last >= tile * TR) kend = p.causal ? min(max(last + diff + 1, 0), kvlen) : kvlen;
   const int ntile = (kend + BN - 1) / BN, per = (ntile + p.splits - 1) / p.splits;
-  const int t0 = min((int)blockIdx.y * per, ntile), t1 = min(t0 + per, ntile);
+  const int t0 = min(u.split * per, ntile), t1 = min(t0 + per, ntile);
 
   AtLoader<D, BN, NW> lk, lv;
   lk.init(p.sk[1], p.D, wave, lane);
@@ -542,6 +597,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
       ring_barrier();
       at_exchange<2, NT, DW>(xbuf, wave, lane, dp);
     }
+    AtTrAhead<D, DT, 1> ka;
+    ka.start(smem, tr_at + stage);
     const bool mask = key0 + BN > wmin;
     at_s8 ds[NT];
 #pragma unroll
@@ -565,9 +622,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
     for (int nt = 0; nt < NT; ++nt) ds[nt] = at_pack8(s[0][nt] * dp[0][nt], s[1][nt] * dp[1][nt]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const at_s8 a = at_tr<D>(smem, (tr_at + stage) ^ (dt << 5));
+      const at_s8 a = ka.take(smem, tr_at + stage, dt);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, ds[nt], acc[dt][nt]);
+      at_order();
     }
   }
 #pragma unroll
@@ -581,7 +639,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
       if (d >= p.D) continue;
       const at_f4 a = any ? acc[dt][nt] : at_f4{0.f, 0.f, 0.f, 0.f};
       if (p.splits > 1)
-        *reinterpret_cast<at_f4*>(p.part + blockIdx.y * ((long long)p.B * p.Nq * p.H * p.D) + at + d) = a;
+        *reinterpret_cast<at_f4*>(p.part + u.split * ((long long)p.B * p.Nq * p.H * p.D) + at + d) = a;
       else
         at_store4(p.dq + at + d, a[0] * p.scale, a[1] * p.scale, a[2] * p.scale, a[3] * p.scale);
     }
@@ -603,8 +661,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_kv_kernel(const AttnArgs 
   constexpr int V_AT = 4 * TILE;
   char* stats = smem + V_AT + (VL ? TK * D * 2 : 0);
   char* xbuf = stats + 512;
-  const int u = at_unit(blockIdx.x, gridDim.x);
-  const int tile = u % p.tiles, hk = (u / p.tiles) % p.Hk, b = u / p.tiles / p.Hk;
+  const AtUnit u = at_unit(blockIdx.x, p.tiles, p.splits, p.Hk * p.B, p.causal);
+  const int tile = u.tile, hk = u.head % p.Hk, b = u.head / p.Hk;   // under a causal mask the first keys have the most queries
   const int G = p.H / p.Hk;
   const int qlen = at_len(p.q_len, b, p.Nq), kvlen = at_len(p.kv_len, b, p.Nk), diff = kvlen - qlen;
   const int key_first = tile * TK, wkey = key_first + wr * NT * 16;
@@ -629,7 +687,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_kv_kernel(const AttnArgs 
   const int nq = key_first < kvlen ? (qlen + BQ - 1) / BQ : 0;
   const int qt0 = p.causal ? min(max(key_first - diff, 0) / BQ, nq) : 0;
   const int per_head = nq - qt0, n_it = per_head * G, per = (n_it + p.splits - 1) / p.splits;
-  const int it0 = min((int)blockIdx.y * per, n_it), it1 = min(it0 + per, n_it);
+  const int it0 = min(u.split * per, n_it), it1 = min(it0 + per, n_it);
 
   AtLoader<D, BQ, NW> lq, ld;
   lq.init(p.sq[1], p.D, wave, lane);
@@ -757,7 +815,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_kv_kernel(const AttnArgs 
       if (d >= p.D) continue;
       const at_f4 a = ak[dt][nt], w = av[dt][nt];
       if (p.splits > 1) {
-        float* dst = p.part + (long long)blockIdx.y * 2 * n_all + at + d;
+        float* dst = p.part + (long long)u.split * 2 * n_all + at + d;
         *reinterpret_cast<at_f4*>(dst) = a;
         *reinterpret_cast<at_f4*>(dst + n_all) = w;
       } else {
@@ -768,14 +826,19 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_kv_kernel(const AttnArgs 
   }
 }
 
-// dst = bf16(mul * sum over splits), in split order; four elements per thread, n % 8 == 0
+// dst = bf16(mul * sum over splits), in split order; four elements per thread, n % 8 == 0.  The first n of a split's part go
+// to dst0 with mul0, the n behind them (blockIdx.y = 1) to dst1 with mul1.
 __global__ __launch_bounds__(256) void attn_reduce_kernel(const float* __restrict__ part, long long split_stride, int splits,
-                                                          long long n, float mul, uint16_t* __restrict__ dst) {
+                                                          long long n, float mul0, uint16_t* __restrict__ dst0, float mul1,
+                                                          uint16_t* __restrict__ dst1) {
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
+  const float* src = part + (blockIdx.y ? n : 0) + i;
   at_f4 a = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; ++s) a += *reinterpret_cast<const at_f4*>(part + s * split_stride + i);
-  at_store4(dst + i, a[0] * mul, a[1] * mul, a[2] * mul, a[3] * mul);
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) a += *reinterpret_cast<const at_f4*>(src + s * split_stride);
+  const float mul = blockIdx.y ? mul1 : mul0;
+  at_store4((blockIdx.y ? dst1 : dst0) + i, a[0] * mul, a[1] * mul, a[2] * mul, a[3] * mul);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -810,16 +873,20 @@ static AttnPlan at_plan(const trace_attention_desc* d) {
   pl.pack = small ? G : 1;
   pl.units = d->heads / pl.pack;
   pl.tile_rows = small ? 16 : pl.D <= 128 ? 128 : 64;
+  // head_dim 512, one workgroup of eight waves per CU: 128 rows with each wave on a whole row where that fills the card (4 x 4 x
+  // 2048 rows: 111 against 133 us), else 64 rows with two waves on each (8 x 784 rows over 196 keys: 22 against 28 us)
+  if (pl.D == 512 && !small && (long long)ceil_div(d->q_rows, 128) * d->heads * d->batch >= AT_CUS) pl.tile_rows = 128;
   pl.tiles = ceil_div((long long)pl.pack * d->q_rows, pl.tile_rows);
-  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch, ceil_div(d->k_rows, 32), 4, 2);
+  const int uneven = d->causal ? 2 : 1;   // uneven work: more, shorter workgroups
+  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch, ceil_div(d->k_rows, 32), 4, (pl.D <= 256 ? 2 : 1) * uneven);
   const int bwd_rows = pl.D <= 256 ? 128 : 64;
-  const int waves = d->causal ? 4 : 2;   // causal work is uneven: more, shorter workgroups
+  const int per_cu = (pl.D <= 128 ? 2 : 1) * uneven;   // workgroups that a CU holds, by their LDS
   pl.q_rows = bwd_rows;
   pl.q_tiles = ceil_div(d->q_rows, pl.q_rows);
-  pl.q_splits = at_splits((long long)pl.q_tiles * d->heads * d->batch, ceil_div(d->k_rows, 32), 4, 2);
+  pl.q_splits = at_splits((long long)pl.q_tiles * d->heads * d->batch, ceil_div(d->k_rows, 32), 4, per_cu);
   pl.k_rows = pl.D <= 256 ? 128 : 64;
   pl.k_tiles = ceil_div(d->k_rows, pl.k_rows);
-  pl.k_splits = at_splits((long long)pl.k_tiles * d->kv_heads * d->batch, ceil_div(d->q_rows, 32) * G, 4, waves);
+  pl.k_splits = at_splits((long long)pl.k_tiles * d->kv_heads * d->batch, ceil_div(d->q_rows, 32) * G, 4, per_cu);
   return pl;
 }
 
@@ -867,7 +934,7 @@ static bool at_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <int D, int NT, int NW, int DW, int BN> static int at_launch_fwd(const AttnArgs& a, hipStream_t st) {
   const int lds = 4 * BN * D * 2 + (DW > 1 ? NW * (BN / 16) * NT * 1024 : 0);
-  const dim3 grid((unsigned)a.tiles * a.units * a.B, a.splits);
+  const unsigned grid = (unsigned)a.tiles * a.units * a.B * a.splits;
   if (a.o_rest) {
     TRACE_LDS_OPT_IN((attn_fwd_kernel<D, NT, NW, DW, BN, true>), lds, "attention");
     attn_fwd_kernel<D, NT, NW, DW, BN, true><<<grid, 64 * NW, lds, st>>>(a);
@@ -880,13 +947,13 @@ template <int D, int NT, int NW, int DW, int BN> static int at_launch_fwd(const 
 template <int D, int NT, int NW, int DW> static int at_launch_q(const AttnArgs& a, hipStream_t st) {
   const int lds = 4 * 32 * D * 2 + (DW > 1 ? NW * 2 * NT * 1024 : 0);
   TRACE_LDS_OPT_IN((attn_bwd_q_kernel<D, NT, NW, DW>), lds, "attention backward");
-  attn_bwd_q_kernel<D, NT, NW, DW><<<dim3((unsigned)a.tiles * a.H * a.B, a.splits), 64 * NW, lds, st>>>(a);
+  attn_bwd_q_kernel<D, NT, NW, DW><<<(unsigned)a.tiles * a.H * a.B * a.splits, 64 * NW, lds, st>>>(a);
   return 0;
 }
 template <int D, int NT, int NW, int DW> static int at_launch_kv(const AttnArgs& a, hipStream_t st) {
   const int lds = 4 * 32 * D * 2 + 512 + (DW > 1 ? NW * 2 * NT * 1024 : NW * NT * 16 * D * 2);
   TRACE_LDS_OPT_IN((attn_bwd_kv_kernel<D, NT, NW, DW>), lds, "attention backward");
-  attn_bwd_kv_kernel<D, NT, NW, DW><<<dim3((unsigned)a.tiles * a.Hk * a.B, a.splits), 64 * NW, lds, st>>>(a);
+  attn_bwd_kv_kernel<D, NT, NW, DW><<<(unsigned)a.tiles * a.Hk * a.B * a.splits, 64 * NW, lds, st>>>(a);
   return 0;
 }
 
@@ -944,16 +1011,15 @@ extern "C" int trace_attention_fwd_bf16(const trace_attention_desc* d, const uin
       case 32: rc = at_launch_fwd<32, 2, 4, 1, 64>(a, st); break;
       case 64: rc = at_launch_fwd<64, 2, 4, 1, 64>(a, st); break;
       case 128: rc = at_launch_fwd<128, 2, 4, 1, 64>(a, st); break;
-      case 256: rc = at_launch_fwd<256, 2, 4, 2, 32>(a, st); break;
-      default: rc = at_launch_fwd<512, 2, 8, 4, 32>(a, st); break;
+      case 256: rc = at_launch_fwd<256, 1, 4, 1, 32>(a, st); break;
+      default: rc = pl.tile_rows == 128 ? at_launch_fwd<512, 1, 8, 1, 32>(a, st) : at_launch_fwd<512, 1, 8, 2, 32>(a, st); break;
     }
   }
   if (rc) return rc;
   if (int e = check_launch("attention")) return e;
   if (pl.splits > 1) {
-    const int grid = ceil_div(rows * (d->head_dim / 4), 256);
-    if (out_rest) attn_combine_kernel<true><<<grid, 256, 0, st>>>(a);
-    else attn_combine_kernel<false><<<grid, 256, 0, st>>>(a);
+    if (out_rest) attn_combine_kernel<true><<<(unsigned)rows, 256, 0, st>>>(a);
+    else attn_combine_kernel<false><<<(unsigned)rows, 256, 0, st>>>(a);
     return check_launch("attention combine");
   }
   return 0;
@@ -1012,14 +1078,14 @@ extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uin
       case 32: rc = at_launch_q<32, 2, 4, 1>(a, st); break;
       case 64: rc = at_launch_q<64, 2, 4, 1>(a, st); break;
       case 128: rc = at_launch_q<128, 2, 4, 1>(a, st); break;
-      case 256: rc = at_launch_q<256, 2, 8, 2>(a, st); break;
-      default: rc = at_launch_q<512, 2, 8, 4>(a, st); break;
+      case 256: rc = at_launch_q<256, 1, 8, 1>(a, st); break;
+      default: rc = at_launch_q<512, 1, 8, 2>(a, st); break;
     }
     if (rc) return rc;
     if (int e = check_launch("attention backward (dq)")) return e;
     if (pl.q_splits > 1) {
       const long long n = (long long)d->batch * d->q_rows * d->heads * d->head_dim;
-      attn_reduce_kernel<<<ceil_div(n, 1024), 256, 0, st>>>(a.part, n, pl.q_splits, n, d->scale, dq);
+      attn_reduce_kernel<<<ceil_div(n, 1024), 256, 0, st>>>(a.part, n, pl.q_splits, n, d->scale, dq, 0.f, nullptr);
       if (int e = check_launch("attention backward (dq splits)")) return e;
     }
   }
@@ -1037,8 +1103,7 @@ extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uin
     if (int e = check_launch("attention backward (dk, dv)")) return e;
     if (pl.k_splits > 1) {
       const long long n = (long long)d->batch * d->k_rows * d->kv_heads * d->head_dim;
-      attn_reduce_kernel<<<ceil_div(n, 1024), 256, 0, st>>>(a.part, 2 * n, pl.k_splits, n, d->scale, dk);
-      attn_reduce_kernel<<<ceil_div(n, 1024), 256, 0, st>>>(a.part + n, 2 * n, pl.k_splits, n, 1.0f, dv);
+      attn_reduce_kernel<<<dim3(ceil_div(n, 1024), 2), 256, 0, st>>>(a.part, 2 * n, pl.k_splits, n, d->scale, dk, 1.0f, dv);
       if (int e = check_launch("attention backward (dk, dv splits)")) return e;
     }
   }
