@@ -28,6 +28,7 @@ __device__ __attribute__((aligned(256))) const uint4 g_at_zero[16] = {};
 
 constexpr float AT_LOG2E = 1.4426950408889634f, AT_LN2 = 0.6931471805599453f;
 constexpr int AT_CUS = 256;
+constexpr int AT_MAX_SPLITS = 256;   // a thread each in attn_combine_kernel
 
 struct AttnArgs {
   const uint16_t *q, *k, *v, *out, *rest, *dout;
@@ -56,6 +57,11 @@ template <int D> __device__ __forceinline__ int at_key(int r) {
 }
 template <int D> __device__ __forceinline__ int at_off(int r, int chunk) { return r * (2 * D) + ((chunk ^ at_key<D>(r)) << 4); }
 
+template <bool NT> __device__ __forceinline__ void at_glds(const void* g, char* lds) {
+  if constexpr (NT) glds16_nt(g, lds);
+  else glds16(g, lds);
+}
+
 // One wave's share of the LDS-DMA of a ROWS x D tile (whole workgroup: NW waves).  Consecutive loads of a wave are STEP rows
 // apart; where that is a multiple of eight rows the key repeats, and one lane offset serves them all.
 template <int D, int ROWS, int NW> struct AtLoader {
@@ -75,13 +81,14 @@ template <int D, int ROWS, int NW> struct AtLoader {
     }
   }
   // `rows` rows from `base` (uniform); further rows and the columns behind head_dim (`d` of D) read zeros
+  template <bool NT = false>
   __device__ __forceinline__ void issue(char* lds, const uint16_t* base, long long row_stride, int rows, int d, int wave, int lane) const {
     if (INST < NW && wave >= INST) return;
     const char* b = reinterpret_cast<const char*>(base);
     const long long step = M == 1 ? STEP * row_stride * 2 : 0;
     if (rows >= ROWS && d == D) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) glds16(b + j * step + off[M == 1 ? 0 : j], lds + (j * NW + wave) * 1024);
+      for (int j = 0; j < N; ++j) at_glds<NT>(b + j * step + off[M == 1 ? 0 : j], lds + (j * NW + wave) * 1024);
       return;
     }
     const char* zero = reinterpret_cast<const char*>(g_at_zero);
@@ -89,7 +96,7 @@ template <int D, int ROWS, int NW> struct AtLoader {
     for (int j = 0; j < N; ++j) {
       const int row = ((j * NW + wave) * 64 + lane) / CPR;
       const bool ok = ((colok >> (M == 1 ? 0 : j)) & 1u) && row < rows;
-      glds16(ok ? b + j * step + off[M == 1 ? 0 : j] : zero, lds + (j * NW + wave) * 1024);
+      at_glds<NT>(ok ? b + j * step + off[M == 1 ? 0 : j] : zero, lds + (j * NW + wave) * 1024);
     }
   }
 };
@@ -153,17 +160,18 @@ __device__ __forceinline__ at_f4 at_mfma(const at_s8& a, const at_s8& b, const a
 // (head, split, tile) units, so the tiles that read one head's other operand share an L2.  `uneven`: under a causal mask a
 // tile's work falls with its index (the caller counts from the longest); tile 0 of all heads and splits goes first then, so that
 // short ones fill the end: 2 x 4096 x 16 heads x 128, forward 211 -> 166 us, backward 566 -> 455 us.
+// `spread`: single row tiles share nothing; their splits go round all XCDs, or a long batch entry would keep one of them busy alone.
 struct AtUnit {
   int tile, split, head;   // head: of all batches
 };
-__device__ __forceinline__ AtUnit at_unit(int lin, int tiles, int splits, int heads, bool uneven) {
+__device__ __forceinline__ AtUnit at_unit(int lin, int tiles, int splits, int heads, bool uneven, bool spread = false) {
   const int x = lin & 7, hs = heads * splits;
   int t, h;
-  if (!uneven) {
+  if (!uneven && !spread) {
     const int total = tiles * hs, per = total >> 3, rem = total & 7, u = x * per + min(x, rem) + (lin >> 3);
     t = u % tiles;
     h = u / tiles;
-  } else if ((hs & 7) == 0) {   // neighbouring heads on one XCD
+  } else if ((hs & 7) == 0 && !spread) {   // neighbouring heads on one XCD
     const int hx = hs >> 3, i = lin >> 3;
     t = i / hx;
     h = x * hx + i % hx;
@@ -273,10 +281,11 @@ template <int D, int NT, int NW, int DW, int BN, bool FINE>
 __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) {
   constexpr int TR = NW / DW * NT * 16, KC = D / 32 / DW, DT = D / 16 / DW, ST = BN / 16;
   constexpr int TILE = BN * D * 2;
+  constexpr bool SMALL = TR == 16;   // one row tile: its keys are read once, past the caches
   extern __shared__ __attribute__((aligned(16))) char smem[];   // two stages of [K tile][V tile], exchange buffer
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wd = wave % DW, wr = wave / DW;
-  const AtUnit u = at_unit(blockIdx.x, p.tiles, p.splits, p.units * p.B, p.causal);
+  const AtUnit u = at_unit(blockIdx.x, p.tiles, p.splits, p.units * p.B, p.causal, SMALL);
   const int tile = p.causal ? p.tiles - 1 - u.tile : u.tile;
   const int unit = u.head % p.units, b = u.head / p.units;
   const int G = p.H / p.Hk, hk = unit * p.pack / G;
@@ -313,7 +322,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
     const int last = min((tile + 1) * TR, qlen) - 1;
     if (last >= tile * TR) kend = p.causal ? min(max(last + diff + 1, 0), kvlen) : kvlen;
   }
-  const int ntile = (kend + BN - 1) / BN, per = (ntile + p.splits - 1) / p.splits;
+  // a split's share: of the keys in sight, or, for single row tiles, of the longest batch entry's keys, so that entries of
+  // different lengths make shares of one size
+  const int ntile = (kend + BN - 1) / BN, per = ((SMALL ? (p.Nk + BN - 1) / BN : ntile) + p.splits - 1) / p.splits;
   const int t0 = min(u.split * per, ntile), t1 = min(t0 + per, ntile);
 
   AtLoader<D, BN, NW> lk, lv;
@@ -323,8 +334,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
   const uint16_t* vb = p.v + b * p.sv[0] + hk * p.sv[2];
   auto issue = [&](int t) {
     const int st = ((t - t0) & 1) * (2 * TILE), k0 = t * BN;
-    lk.issue(smem + st, kb + k0 * p.sk[1], p.sk[1], kend - k0, p.D, wave, lane);
-    lv.issue(smem + st + TILE, vb + k0 * p.sv[1], p.sv[1], kend - k0, p.D, wave, lane);
+    lk.template issue<SMALL>(smem + st, kb + k0 * p.sk[1], p.sk[1], kend - k0, p.D, wave, lane);
+    lv.template issue<SMALL>(smem + st + TILE, vb + k0 * p.sv[1], p.sv[1], kend - k0, p.D, wave, lane);
   };
   const int row_at = at_row_base<D>(lane) ^ (wd * KC << 6), tr_at = (at_tr_base<D>(lane) ^ (wd * DT << 5)) + TILE;
 
@@ -440,24 +451,31 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
   }
 }
 
-// out / lse of a row from its splits' (max, sum, unnormalised out).  A workgroup per row: a wave turns the splits' statistics
-// into weights (at most 64 splits), then groups of D / 4 threads add strided lists of splits, and the first group adds the groups.
+// out / lse of a row from its splits' (max, sum, unnormalised out).  A workgroup per row: a thread per split (AT_MAX_SPLITS at
+// most) turns the statistics into weights, then groups of D / 4 threads add strided lists of splits, and the first group adds the
+// groups.
 template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs p) {
-  __shared__ float weight[64];
+  __shared__ float weight[AT_MAX_SPLITS], part[2][4];
   __shared__ at_f4 red[256];
-  const int tid = threadIdx.x, lane = tid & 63, dq = p.D >> 2, groups = min(256 / dq, p.splits);
+  const int tid = threadIdx.x, wave = tid >> 6, dq = p.D >> 2, groups = min(256 / dq, p.splits);
   const long long rows = (long long)p.B * p.H * p.Nq, row = blockIdx.x;
-  if (tid < 64) {
-    const float2 ml = lane < p.splits ? p.part_ml[lane * rows + row] : make_float2(-INFINITY, 0.f);
+  {
+    const float2 ml = tid < p.splits ? p.part_ml[tid * rows + row] : make_float2(-INFINITY, 0.f);
     float mx = ml.x;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    if ((tid & 63) == 0) part[0][wave] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(part[0][0], part[0][1]), fmaxf(part[0][2], part[0][3]));
     const float w = ml.y > 0.f ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.f;
     float sum = w * ml.y;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
-    weight[lane] = sum > 0.f ? w / sum : 0.f;
-    if (lane == 0 && p.lse) p.lse[row] = sum > 0.f ? (mx + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
+    if ((tid & 63) == 0) part[1][wave] = sum;
+    __syncthreads();
+    sum = (part[1][0] + part[1][1]) + (part[1][2] + part[1][3]);
+    weight[tid] = sum > 0.f ? w / sum : 0.f;
+    if (tid == 0 && p.lse) p.lse[row] = sum > 0.f ? (mx + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
   }
   __syncthreads();
   const int grp = tid / dq, d = (tid - grp * dq) * 4;
@@ -859,7 +877,7 @@ static int at_splits(long long groups, int iters, int min_iters, int per_cu) {
   long long s = (per_cu * AT_CUS + groups - 1) / groups;
   const long long most = iters / min_iters;
   if (s > most) s = most;
-  if (s > 64) s = 64;
+  if (s > AT_MAX_SPLITS) s = AT_MAX_SPLITS;
   return s < 1 ? 1 : (int)s;
 }
 
@@ -878,7 +896,8 @@ static AttnPlan at_plan(const trace_attention_desc* d) {
   if (pl.D == 512 && !small && (long long)ceil_div(d->q_rows, 128) * d->heads * d->batch >= AT_CUS) pl.tile_rows = 128;
   pl.tiles = ceil_div((long long)pl.pack * d->q_rows, pl.tile_rows);
   const int uneven = d->causal ? 2 : 1;   // uneven work: more, shorter workgroups
-  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch, ceil_div(d->k_rows, 32), 4, (pl.D <= 256 ? 2 : 1) * uneven);
+  const int held = small ? (pl.D <= 128 ? 5 : pl.D == 256 ? 2 : 1) : (pl.D <= 256 ? 2 : 1) * uneven;   // workgroups that a CU holds, by their LDS
+  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch, ceil_div(d->k_rows, 32), 4, held);
   const int bwd_rows = pl.D <= 256 ? 128 : 64;
   const int per_cu = (pl.D <= 128 ? 2 : 1) * uneven;   // workgroups that a CU holds, by their LDS
   pl.q_rows = bwd_rows;

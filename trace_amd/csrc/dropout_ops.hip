@@ -52,69 +52,74 @@ template <typename T> __device__ __forceinline__ T drop_put(float v) {
   else return f32_to_bf16(v);
 }
 
-// a thread per counter block of eight elements; the block behind the last whole one is done element by element
+constexpr int DROP_U = 2;   // counter blocks of eight elements per thread, all loaded before the first is drawn
+
+template <typename T> struct DropVec {   // eight elements
+  uint4 w[sizeof(T) / 2];
+};
+
+// A workgroup per DROP_U x 256 counter blocks; the elements behind the last whole block are done one by one.
 template <typename T, bool BWD>
 __global__ __launch_bounds__(256) void dropout_act_kernel(const DropArgs p) {
   const uint64_t off = p.offset + (p.step ? (uint64_t)*p.step : 0);
-  const long long blocks = (p.n + 7) >> 3, stride = (long long)gridDim.x * 256;
+  const long long whole = p.n >> 3, b0 = (long long)blockIdx.x * (DROP_U * 256) + threadIdx.x;
   const bool need_x = !BWD || p.act;
   const float low = (p.act & TRACE_EPI_RELU) ? 0.f : (p.act & TRACE_EPI_LEAKY) ? 0.1f : 1.f;
-  for (long long b = (long long)blockIdx.x * 256 + threadIdx.x; b < blocks; b += stride) {
-    const long long i0 = b * 8;
-    const int cnt = (int)min((long long)8, p.n - i0);
-    const T *xp = static_cast<const T*>(p.x) + i0, *gp = static_cast<const T*>(p.dy) + i0;
-    T* op = static_cast<T*>(p.out) + i0;
-    T xv[8], gv[8], ov[8];
-    if (cnt == 8) {
-      if (need_x) {
-        if constexpr (sizeof(T) == 2) {
-          *reinterpret_cast<uint4*>(xv) = *reinterpret_cast<const uint4*>(xp);
-        } else {
-          reinterpret_cast<uint4*>(xv)[0] = reinterpret_cast<const uint4*>(xp)[0];
-          reinterpret_cast<uint4*>(xv)[1] = reinterpret_cast<const uint4*>(xp)[1];
-        }
-      }
-      if (BWD) {
-        if constexpr (sizeof(T) == 2) {
-          *reinterpret_cast<uint4*>(gv) = *reinterpret_cast<const uint4*>(gp);
-        } else {
-          reinterpret_cast<uint4*>(gv)[0] = reinterpret_cast<const uint4*>(gp)[0];
-          reinterpret_cast<uint4*>(gv)[1] = reinterpret_cast<const uint4*>(gp)[1];
-        }
-      }
+  const DropVec<T>*xp = static_cast<const DropVec<T>*>(p.x), *gp = static_cast<const DropVec<T>*>(p.dy);
+  auto one = [&](float x, float g, uint32_t piece) {
+    float v;
+    if (BWD) {
+      v = g * p.scale;
+      if (p.act && !(x > 0.f)) v *= low;
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (need_x && e < cnt) xv[e] = xp[e];
-        if (BWD && e < cnt) gv[e] = gp[e];
-      }
+      v = x * p.scale;
+      if (p.act) v = v < 0.f ? v * low : v;   // NaN stays
     }
+    return piece < p.threshold ? 0.f : v;
+  };
+  DropVec<T> xv[DROP_U], gv[DROP_U];
+#pragma unroll
+  for (int u = 0; u < DROP_U; ++u) {
+    const long long b = b0 + u * 256;
+    if (b < whole) {
+      if (need_x) xv[u] = xp[b];
+      if (BWD) gv[u] = gp[b];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < DROP_U; ++u) {
+    const long long b = b0 + u * 256;
+    if (b > whole) break;
     uint32_t w[4];
     drop_pieces((uint64_t)b, off, p.seed, w);
+    if (b < whole) {
+      DropVec<T> o;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t piece = (e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
-      float v;
-      if (BWD) {
-        v = drop_get<T>(gv[e]) * p.scale;
-        if (p.act && !(drop_get<T>(xv[e]) > 0.f)) v *= low;
-      } else {
-        v = drop_get<T>(xv[e]) * p.scale;
-        if (p.act) v = v < 0.f ? v * low : v;   // NaN stays
+      for (int e = 0; e < 8; e += 2) {
+        float x0 = 0.f, x1 = 0.f, g0 = 0.f, g1 = 0.f;
+        const uint32_t *xw = &xv[u].w[0].x, *gw = &gv[u].w[0].x;
+        uint32_t* ow = &o.w[0].x;
+        if constexpr (sizeof(T) == 2) {
+          if (need_x) x0 = __uint_as_float(xw[e / 2] << 16), x1 = __uint_as_float(xw[e / 2] & 0xffff0000u);
+          if (BWD) g0 = __uint_as_float(gw[e / 2] << 16), g1 = __uint_as_float(gw[e / 2] & 0xffff0000u);
+          ow[e / 2] = pack_bf16x2(one(x0, g0, w[e / 2] & 0xffffu), one(x1, g1, w[e / 2] >> 16));
+        } else {
+          if (need_x) x0 = __uint_as_float(xw[e]), x1 = __uint_as_float(xw[e + 1]);
+          if (BWD) g0 = __uint_as_float(gw[e]), g1 = __uint_as_float(gw[e + 1]);
+          ow[e] = __float_as_uint(one(x0, g0, w[e / 2] & 0xffffu));
+          ow[e + 1] = __float_as_uint(one(x1, g1, w[e / 2] >> 16));
+        }
       }
-      ov[e] = drop_put<T>(piece < p.threshold ? 0.f : v);
-    }
-    if (cnt == 8) {
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(op) = *reinterpret_cast<const uint4*>(ov);
-      } else {
-        reinterpret_cast<uint4*>(op)[0] = reinterpret_cast<const uint4*>(ov)[0];
-        reinterpret_cast<uint4*>(op)[1] = reinterpret_cast<const uint4*>(ov)[1];
-      }
+      static_cast<DropVec<T>*>(p.out)[b] = o;
     } else {
+      const T *xt = static_cast<const T*>(p.x) + b * 8, *gt = static_cast<const T*>(p.dy) + b * 8;
+      T* ot = static_cast<T*>(p.out) + b * 8;
+      const int cnt = (int)(p.n - b * 8);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (e < cnt) op[e] = ov[e];
+        if (e < cnt)
+          ot[e] = drop_put<T>(one(need_x ? drop_get<T>(xt[e]) : 0.f, BWD ? drop_get<T>(gt[e]) : 0.f,
+                                  (e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu));
     }
   }
 }
@@ -141,8 +146,9 @@ static int drop_call(bool backward, const T* x, const T* dy, long long n, int th
   a.offset = offset;
   a.step = step;
   a.act = act;
-  const long long wg = ((n + 7) / 8 + 255) / 256;
-  const unsigned grid = (unsigned)(wg < 4096 ? wg : 4096);
+  const long long wg = (n / 8 + 1 + DROP_U * 256 - 1) / (DROP_U * 256);   // a block more for what is behind the whole ones
+  TRACE_REQUIRE(wg < (1ll << 31), "%s: too many elements", what);
+  const unsigned grid = (unsigned)wg;
   if (backward) dropout_act_kernel<T, true><<<grid, 256, 0, (hipStream_t)stream>>>(a);
   else dropout_act_kernel<T, false><<<grid, 256, 0, (hipStream_t)stream>>>(a);
   return check_launch(what);

@@ -548,21 +548,28 @@ __global__ __launch_bounds__(GN_CT) void gn_stats_kernel(const GnArgs p) {
   }
 }
 
-// wave per (group, sample): the chunks' moments, each lane a strided list in order, then pairs of lanes -> stats
-__global__ __launch_bounds__(64) void gn_merge_kernel(const GnArgs p) {
-  const int lane = threadIdx.x, g = blockIdx.x, n = blockIdx.y;
+// workgroup per (group, sample): the chunks' moments, each thread a strided list in order, then pairs of lanes, then the waves
+// -> stats
+__global__ __launch_bounds__(GN_CT) void gn_merge_kernel(const GnArgs p) {
+  __shared__ GnMom wm[GN_CT / 64];
+  const int tid = threadIdx.x, g = blockIdx.x, n = blockIdx.y;
   GnMom m = {0.f, 0.f, 0.f};
-  for (int k = lane; k < p.chunks; k += 64) {
+#pragma unroll 4
+  for (int k = tid; k < p.chunks; k += GN_CT) {
     const float2 o = *reinterpret_cast<const float2*>(p.part + 2 * (((long long)n * p.chunks + k) * p.G + g));
     m = gn_merge(m, {(float)min(p.rows, p.P - k * p.rows) * (float)p.Cg, o.x, o.y});
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const GnMom t = {__shfl_xor(m.n, o), __shfl_xor(m.mean, o), __shfl_xor(m.m2, o)};
-    m = (lane & o) ? gn_merge(t, m) : gn_merge(m, t);   // both lanes the same way round
+    m = (tid & o) ? gn_merge(t, m) : gn_merge(m, t);   // both lanes the same way round
   }
-  if (lane == 0)
+  if ((tid & 63) == 0) wm[tid >> 6] = m;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < GN_CT / 64; ++w) m = gn_merge(m, wm[w]);
     *reinterpret_cast<float2*>(p.stats + 2 * ((long long)n * p.G + g)) = make_float2(m.mean, 1.f / sqrtf(m.m2 / m.n + p.eps));
+  }
 }
 
 template <typename T, int V>
@@ -682,12 +689,14 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_merge_kernel(const GnArgs p) {
     const int j = tid / W, w = tid - j * W, c = g * p.Cg + c0 + w;
     const bool ok = j < J && c0 + w < p.Cg;
     float a = 0.f, b = 0.f;
-    if (ok)
+    if (ok) {
+#pragma unroll 4
       for (int k = j; k < p.chunks; k += J) {
         const float2 s = *reinterpret_cast<const float2*>(p.part + 2 * (((long long)n * p.chunks + k) * p.C + c));
         a += s.x;
         b += s.y;
       }
+    }
     __syncthreads();
     sa[tid] = a;
     sb[tid] = b;
@@ -852,7 +861,7 @@ template <typename T, int V> static int gn_run(const GnArgs& a, const GnPlan& pl
     if (!backward) {
       TRACE_LDS_OPT_IN((gn_stats_kernel<T, V>), 2 * GN_MAX_C * 4 + 4096, "group_norm");
       gn_stats_kernel<T, V><<<grid, GN_CT, lds_s, st>>>(a);
-      gn_merge_kernel<<<dim3(a.G, a.N), 64, 0, st>>>(a);
+      gn_merge_kernel<<<dim3(a.G, a.N), GN_CT, 0, st>>>(a);
       gn_apply_kernel<T, V><<<grid, GN_CT, 0, st>>>(a);
     } else {
       TRACE_LDS_OPT_IN((gn_bwd_sums_kernel<T, V>), 2 * GN_MAX_C * 4 + 4096, "group_norm backward");
