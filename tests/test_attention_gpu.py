@@ -308,3 +308,24 @@ def test_refusals():
                  (do, q, k, v, out.float(), lse, rest), (do, q, k, v, out, lse.double(), rest), (do, q, k, v, out, lse, rest[:1])):
         with pytest.raises(RuntimeError):
             ops.attention_backward(*args)
+
+
+@pytest.mark.parametrize("Nq,Nk", [(1, 40), (1, 3000), (100, 60), (20, 3000)])
+def test_nan_is_not_hidden(Nq, Nk):
+    """a NaN that a row sees reaches its output and its lse, also where the keys are split; other rows do not notice"""
+    from trace_amd import ops
+    q, k, v, do = (t.to(DEV) for t in make(2, Nq, Nk, 2, 2, 64, 21))
+    q[0, Nq // 2, 1] = math.nan
+    for kw in (dict(return_lse=True), dict(for_backward=True)):
+        out, lse = ops.attention(q, k, v, **kw)[:2]
+        bad = torch.zeros((2, 2, Nq), dtype=torch.bool, device=DEV)
+        bad[0, 1, Nq // 2] = True
+        assert torch.equal(lse.isnan(), bad) and torch.equal(out.isnan().all(-1).transpose(1, 2), bad)
+        assert torch.equal(out.isnan().any(-1).transpose(1, 2), bad)
+    q[0, Nq // 2, 1] = 0
+    k[1, Nk - 1, 0, 3] = math.nan
+    out = ops.attention(q, k, v)
+    assert out[1, :, 0].isnan().all() and not out[0].isnan().any() and not out[1, :, 1].isnan().any()
+    # rows that a causal mask keeps from the key
+    out, lse, rest = ops.attention(q, k, v, causal=True, for_backward=True)
+    assert out[1, Nq - 1, 0].isnan().all() and not lse[1, 0, :Nq - 1].isnan().any()

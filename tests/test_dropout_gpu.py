@@ -120,7 +120,7 @@ def test_relation_logits_train():
     r = torch.randn(out.shape).bfloat16().float()
     (out * r.to(DEV)).sum().backward()
     ref, leaves = part.double(), []
-    for x, seq, key in ((sem, m.relation_infer_sem, 11), (spa, m.relation_infer_spa, 10)):
+    for x, seq, key in ((sem, m.relation_infer_sem, 11), (spa, m.relation_infer_spa, 11 + (1 << 63))):
         keep = torch.from_numpy(pieces(np.arange(P * K), key, 3) >= np.uint64(32768)).view(P, K).double()
         x = x.bfloat16().double().requires_grad_(True)
         w = seq[2].weight.detach().cpu().bfloat16().double().requires_grad_(True)

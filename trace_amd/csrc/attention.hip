@@ -427,7 +427,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_fwd_kernel(const AttnArgs p) 
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
     if (row_i[nt] < 0) continue;
-    const bool any = lim[nt] > 0 && sum > 0.f;
+    const bool any = lim[nt] > 0 && !(split && sum == 0.f);   // a split may hold none of the keys that the row sees; NaN counts
     const long long row = ((long long)b * p.H + row_h[nt]) * p.Nq + row_i[nt];
     if (split) {
       const long long rows = (long long)p.B * p.H * p.Nq, at = u.split * rows + row;
@@ -467,15 +467,15 @@ template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_kernel(
     if ((tid & 63) == 0) part[0][wave] = mx;
     __syncthreads();
     mx = fmaxf(fmaxf(part[0][0], part[0][1]), fmaxf(part[0][2], part[0][3]));
-    const float w = ml.y > 0.f ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.f;
+    const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
     float sum = w * ml.y;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
     if ((tid & 63) == 0) part[1][wave] = sum;
     __syncthreads();
     sum = (part[1][0] + part[1][1]) + (part[1][2] + part[1][3]);
-    weight[tid] = sum > 0.f ? w / sum : 0.f;
-    if (tid == 0 && p.lse) p.lse[row] = sum > 0.f ? (mx + __builtin_amdgcn_logf(sum)) * AT_LN2 : -INFINITY;
+    weight[tid] = sum == 0.f ? 0.f : w / sum;
+    if (tid == 0 && p.lse) p.lse[row] = sum == 0.f ? -INFINITY : (mx + __builtin_amdgcn_logf(sum)) * AT_LN2;
   }
   __syncthreads();
   const int grp = tid / dq, d = (tid - grp * dq) * 4;
@@ -494,6 +494,41 @@ template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_kernel(
     const long long b = row / p.Nq / p.H;
     at_store_out<FINE>(p, ((b * p.Nq + i) * p.H + h) * p.D + d, o);
   }
+}
+
+// The same for at most AT_FEW splits: a thread per four columns of a row, all its loads in flight at once.  Thousands of rows come
+// in few splits, and a workgroup each would cost them more than the sums (8000 rows x 128 in 4 splits: FEWUS us).
+constexpr int AT_FEW = 8;
+template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_few_kernel(const AttnArgs p) {
+  const int dq = p.D >> 2;
+  const long long rows = (long long)p.B * p.H * p.Nq, id = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= rows * dq) return;
+  const long long row = id / dq;
+  const int d = (int)(id - row * dq) * 4;
+  float2 ml[AT_FEW];
+  at_f4 v[AT_FEW];
+  float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < AT_FEW; ++s)
+    if (s < p.splits) {
+      ml[s] = p.part_ml[s * rows + row];
+      v[s] = *reinterpret_cast<const at_f4*>(p.part + (s * rows + row) * p.D + d);   // unwritten where the split saw nothing
+    }
+#pragma unroll
+  for (int s = 0; s < AT_FEW; ++s)
+    if (s < p.splits) mx = fmaxf(mx, ml[s].x);
+  at_f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < AT_FEW; ++s)
+    if (s < p.splits && ml[s].y != 0.f) {
+      const float w = __builtin_amdgcn_exp2f(ml[s].x - mx);
+      sum += w * ml[s].y;
+      o += w * v[s];
+    }
+  const int i = (int)(row % p.Nq), h = (int)(row / p.Nq % p.H);
+  const long long b = row / p.Nq / p.H;
+  at_store_out<FINE>(p, ((b * p.Nq + i) * p.H + h) * p.D + d, sum == 0.f ? o : o * (1.f / sum));
+  if (d == 0 && p.lse) p.lse[row] = sum == 0.f ? -INFINITY : (mx + __builtin_amdgcn_logf(sum)) * AT_LN2;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -1037,8 +1072,15 @@ extern "C" int trace_attention_fwd_bf16(const trace_attention_desc* d, const uin
   if (rc) return rc;
   if (int e = check_launch("attention")) return e;
   if (pl.splits > 1) {
-    if (out_rest) attn_combine_kernel<true><<<(unsigned)rows, 256, 0, st>>>(a);
-    else attn_combine_kernel<false><<<(unsigned)rows, 256, 0, st>>>(a);
+    if (pl.splits <= AT_FEW) {
+      const int grid = ceil_div(rows * (d->head_dim / 4), 256);
+      if (out_rest) attn_combine_few_kernel<true><<<grid, 256, 0, st>>>(a);
+      else attn_combine_few_kernel<false><<<grid, 256, 0, st>>>(a);
+    } else if (out_rest) {
+      attn_combine_kernel<true><<<(unsigned)rows, 256, 0, st>>>(a);
+    } else {
+      attn_combine_kernel<false><<<(unsigned)rows, 256, 0, st>>>(a);
+    }
     return check_launch("attention combine");
   }
   return 0;

@@ -1272,11 +1272,11 @@ class Generalized_RCNN(PackedLinears):
         relation_infer_sem(sem) + relation_infer_spa(spatio) (+ so_part), each Dropout -> LeakyReLU(0.1) -> Linear, as
         dropout_act + gemm_nt.  sem / spatio (P, infer) bf16 or f32 features in front of the Dropout -> (P, NUM_PRD_CLASSES)
         f32.  In training mode the masks are functions of (seed, offset + step) - sem draws from `seed`, spatio from
-        `seed` ^ 1 -, so a caller advances `offset` (or the device scalar `step`, for a captured step) every step; in eval
+        `seed` with its top bit flipped -, so a caller advances `offset` (or the device scalar `step`, for a captured step) every step; in eval
         mode nothing is dropped."""
         from . import autograd as tag
         total = None if so_part is None else so_part.float()
-        for x, seq, key in ((sem, self.relation_infer_sem, int(seed)), (spatio, self.relation_infer_spa, int(seed) ^ 1)):
+        for x, seq, key in ((sem, self.relation_infer_sem, int(seed)), (spatio, self.relation_infer_spa, int(seed) ^ 1 << 63)):
             h = tag.dropout_act(x, seq[0].p, key, offset, "leaky", step, training=self.training)
             w, b = seq[2].weight, seq[2].bias
             pad = -w.shape[0] % 8
