@@ -7,7 +7,7 @@
 // Bound by HBM: x once in, y once out (backward: x and dy in, dx out).  Two forms:
 //   * one workgroup per (sample, slab of whole groups) that keeps the slab in registers between the statistics and the
 //     result: everything is read once, one launch.  Taken where the slab fits (P rows of at least 64 contiguous bytes, <=
-//     GN_R 16-byte pieces per thread);
+//     GN_R_FWD / GN_R_BWD 16-byte pieces per thread);
 //   * larger maps in two passes over (sample, chunk of rows), a small merge of the chunks' partial results between them; the
 //     second pass walks the chunks from the last to the first, so that it starts with what the caches still hold.
 // Statistics are merged as (count, mean, sum of squared deviations), never as sum of squares minus squared sum: a map whose
@@ -18,7 +18,7 @@
 namespace trace {
 
 constexpr int GN_BT = 512;      // threads of the one-pass form
-constexpr int GN_R = 16;        // 16-byte pieces a thread of it keeps
+constexpr int GN_R_FWD = 32, GN_R_BWD = 16;   // 16-byte pieces (pairs of them) that a thread of it keeps
 constexpr int GN_CT = 256;      // threads of the two-pass form
 constexpr int GN_MAX_C = 8192;
 
@@ -175,7 +175,7 @@ template <int BT, int K> __device__ __forceinline__ void gn_group_sums(float (&v
 // One pass: workgroup (slab of `slab` groups, sample).  Thread = one V-wide column of the slab, rows tid / SW + i RP.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int V, int R>
-__global__ __launch_bounds__(GN_BT) void gn_fwd_slab_kernel(const GnArgs p) {
+__global__ __launch_bounds__(GN_BT, 2) void gn_fwd_slab_kernel(const GnArgs p) {
   using Raw = typename GnVec<T, V>::type;
   __shared__ float red[GN_BT * V];
   __shared__ float mu[GN_BT * V], rs[GN_BT * V];   // per channel of the slab
@@ -194,6 +194,8 @@ __global__ __launch_bounds__(GN_BT) void gn_fwd_slab_kernel(const GnArgs p) {
   const float inv = 1.f / ((float)p.P * (float)p.Cg);
   float mean[V], rstd[V], s[V];
 #pragma unroll
+  for (int v = 0; v < V; ++v) mean[v] = 0.f;
+#pragma unroll
   for (int pass = 0; pass < 2; ++pass) {   // the mean, then the squared deviations from it
 #pragma unroll
     for (int v = 0; v < V; ++v) s[v] = 0.f;
@@ -206,6 +208,7 @@ __global__ __launch_bounds__(GN_BT) void gn_fwd_slab_kernel(const GnArgs p) {
         for (int v = 0; v < V; ++v) {
           const float d = pass ? f[v] - mean[v] : f[v];
           s[v] += pass ? d * d : d;
+          asm volatile("" : "+v"(s[v]));   // one after the other: joined to wide vectors, 32 narrow rows spill
         }
       }
       gn_row_done();
@@ -284,7 +287,7 @@ __device__ __forceinline__ void gn_channel_out(const GnArgs& p, int n, int c, fl
 }
 
 template <typename T, int V, int R>
-__global__ __launch_bounds__(GN_BT) void gn_bwd_slab_kernel(const GnArgs p) {
+__global__ __launch_bounds__(GN_BT, 2) void gn_bwd_slab_kernel(const GnArgs p) {
   using Raw = typename GnVec<T, V>::type;
   __shared__ float ra[GN_BT * V], rb[GN_BT * V];
   const int tid = threadIdx.x, n = blockIdx.y;
@@ -428,6 +431,19 @@ __global__ __launch_bounds__(GN_BT) void gn_bwd_slab_kernel(const GnArgs p) {
 // Two passes: workgroup (chunk of rows, sample), all channels.  Thread = V-wide columns tid % CV (+ GN_CT ..), rows of its
 // own; with C / V <= GN_CT columns RP = GN_CT / CV rows go side by side.
 // ---------------------------------------------------------------------------------------------------------------
+// groups of the V channels from c on: one division
+template <int V> __device__ __forceinline__ void gn_groups(int c, int Cg, int (&g)[V]) {
+  int q = c / Cg, r = c - q * Cg;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    g[v] = q;
+    if (++r == Cg) {
+      r = 0;
+      ++q;
+    }
+  }
+}
+
 struct GnMom {   // count, mean, sum of squared deviations
   float n, mean, m2;
 };
@@ -582,10 +598,12 @@ __global__ __launch_bounds__(GN_CT) void gn_apply_kernel(const GnArgs p) {
   if (rr >= RP) return;
   for (int cv = CV < GN_CT ? tid - rr * CV : tid; cv < CV; cv += CV < GN_CT ? CV : GN_CT) {
     float mean[V], ga[V], be[V];
+    int grp[V];
+    gn_groups<V>(cv * V, p.Cg, grp);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = cv * V + v, g = c / p.Cg;
-      const float2 st = *reinterpret_cast<const float2*>(p.stats + 2 * ((long long)n * p.G + g));
+      const int c = cv * V + v;
+      const float2 st = *reinterpret_cast<const float2*>(p.stats + 2 * ((long long)n * p.G + grp[v]));
       mean[v] = st.x;
       ga[v] = st.y * (p.gamma ? p.gamma[c] : 1.f);
       be[v] = p.beta ? p.beta[c] : 0.f;
@@ -628,12 +646,14 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_sums_kernel(const GnArgs p) {
       const long long base = (long long)n * p.P * p.C + (long long)cv * V;
       const T *x = static_cast<const T*>(p.x) + base, *dy = static_cast<const T*>(p.dy) + base;
       float mean[V], rstd[V], ga[V], be[V], a[V], b[V];
+      int grp[V];
+      gn_groups<V>(cv * V, p.Cg, grp);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int c = cv * V + v;
-        const float* st = p.stats + 2 * ((long long)n * p.G + c / p.Cg);
-        mean[v] = st[0];
-        rstd[v] = st[1];
+        const float2 st = *reinterpret_cast<const float2*>(p.stats + 2 * ((long long)n * p.G + grp[v]));
+        mean[v] = st.x;
+        rstd[v] = st.y;
         ga[v] = p.gamma ? p.gamma[c] : 1.f;
         be[v] = p.beta ? p.beta[c] : 0.f;
         a[v] = b[v] = 0.f;
@@ -754,10 +774,12 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_apply_kernel(const GnArgs p) {
     const T *x = static_cast<const T*>(p.x) + base, *dy = static_cast<const T*>(p.dy) + base;
     T* dx = static_cast<T*>(p.out) + base;
     float mean[V], rstd[V], ga[V], be[V], a[V], b[V];
+    int grp[V];
+    gn_groups<V>(cv * V, p.Cg, grp);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = cv * V + v;
-      const long long at = 2 * ((long long)n * p.G + c / p.Cg);
+      const long long at = 2 * ((long long)n * p.G + grp[v]);
       mean[v] = p.stats[at];
       rstd[v] = p.stats[at + 1];
       a[v] = p.gsum[at];
@@ -801,7 +823,7 @@ struct GnPlan {
   int rows, chunks;
 };
 
-static GnPlan gn_plan(int N, int P, int C, int G, int elem) {
+static GnPlan gn_plan(int N, int P, int C, int G, int elem, bool backward) {
   GnPlan pl = {};
   pl.V = 16 / elem;
   while (C % pl.V) pl.V >>= 1;
@@ -812,9 +834,9 @@ static GnPlan gn_plan(int N, int P, int C, int G, int elem) {
     if (sc * elem < 64 && k < G) continue;
     if (sc / pl.V > GN_BT) break;
     const int rp = GN_BT / (int)(sc / pl.V), pieces = ceil_div(P, rp);
-    if (pieces > GN_R) break;
+    if (pieces > (backward ? GN_R_BWD : GN_R_FWD)) break;
     pl.slab = k;
-    pl.R = pieces <= 4 ? 4 : pieces <= 8 ? 8 : 16;
+    pl.R = pieces <= 4 ? 4 : pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
   }
   // chunks of whole loads (GN_U rows of every thread): as many loads each as leave about 2048 workgroups, eight to a CU
   const int cv = C / pl.V, rp = cv < GN_CT ? GN_CT / cv : 1, unit = GN_U * rp;
@@ -847,7 +869,8 @@ template <typename T, int V> static void gn_run_slab(const GnArgs& a, const GnPl
   else gn_fwd_slab_kernel<T, V, RR><<<grid, GN_BT, 0, st>>>(a)
   if (pl.R == 4) { TRACE_GN_SLAB(4); }
   else if (pl.R == 8) { TRACE_GN_SLAB(8); }
-  else { TRACE_GN_SLAB(16); }
+  else if (pl.R == 16) { TRACE_GN_SLAB(16); }
+  else { gn_fwd_slab_kernel<T, V, GN_R_FWD><<<grid, GN_BT, 0, st>>>(a); }
 #undef TRACE_GN_SLAB
 }
 
@@ -905,7 +928,7 @@ static int gn_call(bool backward, const T* x, const T* dy, int N, long long P, i
     return check_launch(what);
   }
   TRACE_REQUIRE(x && out && stats && (dy || !backward), "%s: null pointer", what);
-  const GnPlan pl = gn_plan(N, (int)P, C, G, sizeof(T));
+  const GnPlan pl = gn_plan(N, (int)P, C, G, sizeof(T), backward);
   size_t csum, gsum, part;
   gn_bytes(pl, N, C, G, backward, &csum, &gsum, &part);
   TRACE_REQUIRE(ws_bytes >= csum + gsum + part && (ws || !(csum + gsum + part)), "%s: workspace of %zu bytes needed", what, csum + gsum + part);
@@ -945,7 +968,7 @@ extern "C" size_t trace_group_norm_workspace_bytes(int N, long long P, int C, in
   size_t most = 0;
   for (int elem = 2; elem <= 4; elem += 2) {   // either element type
     size_t c, g, p;
-    gn_bytes(gn_plan(N, (int)P, C, G, elem), N, C, G, backward != 0, &c, &g, &p);
+    gn_bytes(gn_plan(N, (int)P, C, G, elem, backward != 0), N, C, G, backward != 0, &c, &g, &p);
     if (c + g + p > most) most = c + g + p;
   }
   return most;
