@@ -496,38 +496,36 @@ template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_kernel(
   }
 }
 
-// The same for at most AT_FEW splits: a thread per four columns of a row, all its loads in flight at once.  Thousands of rows come
-// in few splits, and a workgroup each would cost them more than the sums (8000 rows x 128 in 4 splits: FEWUS us).
+// The same for at most AT_FEW splits: a thread per four columns of a row.  Thousands of rows come in few splits, and a workgroup
+// each would cost them more than the sums.
 constexpr int AT_FEW = 8;
 template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_few_kernel(const AttnArgs p) {
-  const int dq = p.D >> 2;
-  const long long rows = (long long)p.B * p.H * p.Nq, id = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= rows * dq) return;
-  const long long row = id / dq;
-  const int d = (int)(id - row * dq) * 4;
+  const int dq = p.D >> 2, sub = threadIdx.x / dq, d = ((int)threadIdx.x - sub * dq) * 4;
+  const int rows = p.B * p.H * p.Nq, row = blockIdx.x * (256 / dq) + sub;   // rows stay below 2^31: at_check
+  if (sub >= 256 / dq || row >= rows) return;
+  const float* src = p.part + (long long)row * p.D + d;
+  const long long step = (long long)rows * p.D;
+  float mx = -INFINITY, w[AT_FEW];
   float2 ml[AT_FEW];
-  at_f4 v[AT_FEW];
-  float mx = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int s = 0; s < AT_FEW; ++s)
-    if (s < p.splits) {
-      ml[s] = p.part_ml[s * rows + row];
-      v[s] = *reinterpret_cast<const at_f4*>(p.part + (s * rows + row) * p.D + d);   // unwritten where the split saw nothing
-    }
+    if (s < p.splits) ml[s] = p.part_ml[(long long)s * rows + row];
 #pragma unroll
   for (int s = 0; s < AT_FEW; ++s)
     if (s < p.splits) mx = fmaxf(mx, ml[s].x);
+  float sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < AT_FEW; ++s) {
+    w[s] = s >= p.splits || ml[s].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[s].x - mx);
+    if (s < p.splits) sum += w[s] * ml[s].y;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   at_f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int s = 0; s < AT_FEW; ++s)
-    if (s < p.splits && ml[s].y != 0.f) {
-      const float w = __builtin_amdgcn_exp2f(ml[s].x - mx);
-      sum += w * ml[s].y;
-      o += w * v[s];
-    }
-  const int i = (int)(row % p.Nq), h = (int)(row / p.Nq % p.H);
-  const long long b = row / p.Nq / p.H;
-  at_store_out<FINE>(p, ((b * p.Nq + i) * p.H + h) * p.D + d, sum == 0.f ? o : o * (1.f / sum));
+    if (w[s] != 0.f) o += (w[s] * inv) * *reinterpret_cast<const at_f4*>(src + s * step);   // else: never written
+  const int i = row % p.Nq, bh = row / p.Nq, h = bh % p.H, b = bh / p.H;
+  at_store_out<FINE>(p, (((long long)b * p.Nq + i) * p.H + h) * p.D + d, o);
   if (d == 0 && p.lse) p.lse[row] = sum == 0.f ? -INFINITY : (mx + __builtin_amdgcn_logf(sum)) * AT_LN2;
 }
 
@@ -1073,7 +1071,7 @@ extern "C" int trace_attention_fwd_bf16(const trace_attention_desc* d, const uin
   if (int e = check_launch("attention")) return e;
   if (pl.splits > 1) {
     if (pl.splits <= AT_FEW) {
-      const int grid = ceil_div(rows * (d->head_dim / 4), 256);
+      const int grid = ceil_div(rows, 256 / (d->head_dim / 4));
       if (out_rest) attn_combine_few_kernel<true><<<grid, 256, 0, st>>>(a);
       else attn_combine_few_kernel<false><<<grid, 256, 0, st>>>(a);
     } else if (out_rest) {
