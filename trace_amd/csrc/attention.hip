@@ -15,6 +15,19 @@
 //
 // Tiles of rows x head_dim go HBM / L2 -> LDS by 16-byte LDS-DMA, two stages deep; rows behind the sequence and columns
 // behind head_dim read a zero page, so nothing behind a length is ever touched.
+//
+// What bounds them at full size is the matrix pipe together with the vector work between its products (an exponential, its
+// scaling and its rounding per score): 2 x 4096 x 16 heads x 128 without a mask runs forward at 900 TFLOP/s, forward for a
+// backward pass at 1070 and backward at 1170 TFLOP/s of the products it executes, where a library matmul of 8192^3 reaches
+// 1190.  LDS reads take 16 % of the cycles and conflicts none; reading fragments further ahead changes nothing.  Three choices
+// made that rate:
+//   * every kernel is compiled for two waves per SIMD (256 registers): with more, hipcc keeps the sums in accumulation
+//     registers and spends hundreds of moves per tile on them (dk / dv 1173 us -> 563 us), and a single spilled register
+//     in the loop waits for the prefetch behind it (563 -> 358 us without);
+//   * 32 columns (queries, or keys) per wave where the sums fit, so a fragment from LDS feeds two products; at head_dim 256
+//     and above 16 columns with the whole row in one wave beat 32 with the row shared by two, whose scores have to meet
+//     in LDS (8 x 3136 x 784 x 256: 60 -> 42 us).  Only the sums of dq, dk / dv over 512 columns need the sharing;
+//   * masks stand behind uniform branches, so tiles inside the sequence pay nothing for them.
 #include "lds_dma.h"
 #include <math.h>
 
@@ -531,7 +544,9 @@ template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_few_ker
 
 // ---------------------------------------------------------------------------------------------------------------
 // dq (and delta).  The same walk as the forward's over key tiles of 32, with two scoring products (q k^T and dout v^T); the
-// second one starts from -delta instead of zero.
+// second one starts from -delta instead of zero.  dS is rounded to bf16 for the product, as P is in the forward kernel.  dq and
+// dk / dv each form P and dS for themselves: seven products instead of the five of one pass, whose dq (or dk, dv) would have to
+// be added up by atomics in whatever order workgroups come.  2 x 4096 x 16 heads x 128, causal: 221 us, dk / dv 299 us.
 // ---------------------------------------------------------------------------------------------------------------
 template <int D, int NT, int NW, int DW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p) {
@@ -904,7 +919,9 @@ struct AttnPlan {
 
 static inline size_t at_align(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Splits so that about `per_cu` workgroups per CU exist, each with at least `min_iters` iterations of its loop.
+// Splits so that about `per_cu` workgroups per CU exist, each with at least `min_iters` iterations of its loop (32 rows): the
+// partial results cost a pass over f32 copies of the output and a launch.  4 x 500 x 4 heads x 128: forward 18.9 us with at least
+// 8, 21.3 with 4, 25.9 with 2; backward 46.3 with 4, 50.0 with 8, 57.4 with 2.
 static int at_splits(long long groups, int iters, int min_iters, int per_cu) {
   if (groups <= 0 || 2 * groups > per_cu * AT_CUS) return 1;
   long long s = (per_cu * AT_CUS + groups - 1) / groups;
@@ -930,7 +947,7 @@ static AttnPlan at_plan(const trace_attention_desc* d) {
   pl.tiles = ceil_div((long long)pl.pack * d->q_rows, pl.tile_rows);
   const int uneven = d->causal ? 2 : 1;   // uneven work: more, shorter workgroups
   const int held = small ? (pl.D <= 128 ? 5 : pl.D == 256 ? 2 : 1) : (pl.D <= 256 ? 2 : 1) * uneven;   // workgroups that a CU holds, by their LDS
-  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch, ceil_div(d->k_rows, 32), 4, held);
+  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch, ceil_div(d->k_rows, 32), small ? 4 : 8, held);
   const int bwd_rows = pl.D <= 256 ? 128 : 64;
   const int per_cu = (pl.D <= 128 ? 2 : 1) * uneven;   // workgroups that a CU holds, by their LDS
   pl.q_rows = bwd_rows;
