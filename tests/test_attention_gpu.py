@@ -329,3 +329,48 @@ def test_nan_is_not_hidden(Nq, Nk):
     # rows that a causal mask keeps from the key
     out, lse, rest = ops.attention(q, k, v, causal=True, for_backward=True)
     assert out[1, Nq - 1, 0].isnan().all() and not lse[1, 0, :Nq - 1].isnan().any()
+
+
+def test_offsets_past_32_bits():
+    """a cache of 2^31 + elements: the key that decides is its last one, in the last head and in the first"""
+    from trace_amd import ops
+    Nk, Hk, D = (1 << 20) + 37, 16, 128
+    k = torch.zeros((1, Nk, Hk, D), dtype=torch.bfloat16, device=DEV)
+    v = torch.ones((1, Nk, Hk, D), dtype=torch.bfloat16, device=DEV)
+    assert k.numel() > 1 << 31
+    q = torch.full((1, 1, 2 * Hk, D), 1.0, dtype=torch.bfloat16, device=DEV)
+    k[0, Nk - 1] = 10.0                                       # score 10 sqrt(128) = 113 against 0: nothing else is left
+    v[0, Nk - 1] = torch.arange(Hk, device=DEV).view(Hk, 1).to(torch.bfloat16)
+    out, lse, rest = ops.attention(q, k, v, for_backward=True)
+    want = torch.arange(Hk, device=DEV).repeat_interleave(2).view(1, 1, 2 * Hk, 1).expand_as(out).float()
+    assert torch.equal(out.float(), want)
+    cut = torch.tensor([Nk - 1], dtype=torch.int32, device=DEV)
+    assert torch.equal(ops.attention(q, k, v, kv_len=cut), torch.ones_like(out))      # a mean of equal values
+    del out, lse, rest
+    # forty rows instead of one: the tiled form, and its backward pass over the same keys
+    q = torch.full((1, 40, Hk, D), 1.0, dtype=torch.bfloat16, device=DEV)
+    res = ops.attention(q, k, v, for_backward=True)
+    assert torch.equal(res[0].float(), torch.arange(Hk, device=DEV).view(1, 1, Hk, 1).expand_as(q).float())
+    dq, dk, dv = ops.attention_backward(torch.ones_like(q), q, k, v, *res)
+    assert torch.equal(dv[0, Nk - 1], torch.full((Hk, D), 40.0, dtype=torch.bfloat16, device=DEV)) and not dv[0, :Nk - 1].any()
+    assert not dk[0, :Nk - 1].any()
+
+
+def test_calls_at_once_on_two_streams():
+    """split calls have partial results in scratch: two at once on two streams give what they give alone"""
+    from trace_amd import ops
+    sets = [[t.to(DEV) for t in make(2, 40, 3000, 2, 2, 128, s)] for s in (31, 32)]
+    want = []
+    for q, k, v, do in sets:
+        res = ops.attention(q, k, v, for_backward=True)
+        want.append(res + ops.attention_backward(do, q, k, v, *res))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        got = []
+        for st, (q, k, v, do) in zip(streams, sets):
+            with torch.cuda.stream(st):
+                res = ops.attention(q, k, v, for_backward=True)
+                got.append(res + ops.attention_backward(do, q, k, v, *res))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))

@@ -345,3 +345,24 @@ def test_refusals():
     for args in ((x[:1], x, st, 2), (x.bfloat16(), x, st, 2), (x, x, st[:1], 2), (x, x, st.double(), 2), (x, x, st, 4)):
         with pytest.raises(RuntimeError):
             ops.group_norm_act_backward(*args)
+
+
+def test_offsets_past_32_bits():
+    """2^31 + elements; the last sample by itself gives the same bits"""
+    from trace_amd import ops
+    x = torch.empty((3, 2800001, 256), dtype=torch.bfloat16, device=DEV)
+    assert x.numel() > 1 << 31
+    x.normal_()
+    x[2] += 3
+    y, st = ops.group_norm_act(x, 32, act="silu", return_stats=True)
+    assert abs(float(st[2, :, 0].mean()) - 3) < 1e-2 and abs(float(st[0, :, 0].mean())) < 1e-2
+    tail = x[2, -4:].float()
+    z = (tail - st[2, :, 0].repeat_interleave(8)) * st[2, :, 1].repeat_interleave(8)
+    want = z * torch.sigmoid(z)
+    assert float((y[2, -4:].float() - want).abs().max()) <= 2.0 ** -8 * float(want.abs().max()) + 1e-5
+    del y
+    dx, dg, db = ops.group_norm_act_backward(x, x, st, 32)
+    # dy = x: dbeta = sum of x, dgamma = sum of x xh; xh has mean 0 and variance 1 over a group, so dx is near 0
+    assert float(dx[2, -1000:].float().abs().max()) < 0.1
+    n = x.shape[1]
+    assert abs(float(db.mean()) / n - 3) < 0.05

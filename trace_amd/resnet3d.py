@@ -117,7 +117,7 @@ class ConvModule(nn.Module):
             y = tag.conv3d(x, w.permute(0, 2, 3, 4, 1).reshape(cout, -1), None if c.bias is None else c.bias.float(),
                            c.kernel_size, c.stride, c.padding, c.dilation, relu=False)
             relu = self.with_activation if relu is None else relu
-            return tag.group_norm_act(y, gn.num_groups, gn.weight, gn.bias, gn.eps, "relu" if relu else None)
+            return tag.group_norm_act(y, gn.num_groups, gn.weight.float(), gn.bias.float(), gn.eps, "relu" if relu else None)
         if self.with_norm and self.bn.training:
             # batch statistics (the reference's I3D config trains with norm_eval=False: lib/i3d/resnet3d.py:804-811 leaves
             # the BatchNorm3d of the unfrozen stages in training mode): the raw convolution on the HIP kernel, then
