@@ -196,6 +196,17 @@ def test_no_keys_no_rows():
     assert ops.attention(q, k, v).shape == (0, 4, 2, 64)
 
 
+@pytest.mark.parametrize("Nq,Nk", [(5, 0), (0, 5)])
+def test_empty_views(Nq, Nk):
+    """operands without elements, cut out of memory whose strides the kernels do not take"""
+    from trace_amd import ops
+    q, k, v, do = (torch.ones((2, n, h, 68), dtype=torch.bfloat16, device=DEV)[..., :64] for n, h in ((Nq, 2), (Nk, 1), (Nk, 1), (Nq, 2)))
+    out, lse, rest = ops.attention(q, k, v, for_backward=True)
+    assert out.shape == (2, Nq, 2, 64) and not out.any()
+    for t, g in zip((q, k, v), ops.attention_backward(do, q, k, v, out, lse, rest)):
+        assert g.shape == t.shape and not g.any()
+
+
 def test_lengths_are_clamped():
     from trace_amd import ops
     q, k, v, _ = (t.to(DEV) for t in make(2, 9, 20, 2, 2, 64, 5))

@@ -977,8 +977,10 @@ def _attn_operand(t, name):
 
 
 def _attn_strides(t):
-    # a dimension of one element may carry any stride: it is never stepped over
+    # a dimension of one element may carry any stride, and so may a tensor without elements: neither is ever stepped over
     b, n, h, _ = t.shape
+    if not (b and n):
+        return (0, 0, 0)
     s = t.stride()
     return (s[0] if b > 1 else 0, s[1] if n > 1 else 0, s[2] if h > 1 else 0)
 
@@ -1015,7 +1017,7 @@ def attention(q, k, v, scale=None, causal=False, q_len=None, kv_len=None, return
     that count (None: all; values are clamped to 0 .. N); causal: query i sees key j <= i + kv_len - q_len.  A row behind q_len
     or without a key to see is zero; rows behind a length are never read.  D % 8 == 0, 8 .. 512; the operands' rows may be
     strided (views of a packed projection are taken as they are, other layouts are copied).  Keys and values in front of
-    kv_len must be finite, also those that `causal` hides from some rows.
+    kv_len must be finite, also those that `causal` hides from some rows; for the backward pass so must q and dout in front of q_len.
     return_lse: -> (out, lse), lse (B,H,Nq) f32 the log-sum-exp of each row's scaled scores, -inf where it sees no key.
     for_backward: -> (out, lse, rest), what `attention_backward` takes; rest is a second tensor like out, what rounding lost."""
     q, k, v = _attn_operand(q, "q"), _attn_operand(k, "k"), _attn_operand(v, "v")
