@@ -556,7 +556,8 @@ int trace_upload_slots(const void* pinned, size_t slot_bytes, unsigned* counter,
  *            bf16, with the probabilities carried to 16 bits more - the backward pass needs it, because dout . out is the
  *            difference it takes from every dout . v.  Rows i >= q_len and rows that see no key: out = 0, lse = -inf, no gradient.
  *            Operand rows behind q_len / kv_len are never read; rows of dk / dv behind kv_len and of dq behind q_len are
- *            written as zeros.  Keys and values in front of kv_len have to be finite also where `causal` hides them.
+ *            written as zeros.  Keys and values in front of kv_len have to be finite also where `causal` hides them, and for the
+ *            backward pass q and dout in front of q_len also in rows that see no key.
  * Nothing is summed by atomics: equal calls give equal bits.  workspace: trace_attention_{fwd,bwd}_workspace_bytes(desc)
  * bytes, 256-aligned (0: may be NULL); it is free again when the call's work on `stream` has ended. */
 typedef struct {

@@ -17,6 +17,10 @@ folded into the weights in eval mode, torch's batch_norm over the raw conv outpu
 
 Softmax attention, group norm + activation and dropout + activation have kernels of their own for both directions
 (csrc/attention.hip, norm_ops.hip, dropout_ops.hip); their wrappers stand at the end.
+
+Capturing a backward pass into a graph: let go of every result of an eager pass over the same leaves first (or take fresh
+leaves).  torch keeps a leaf's gradient node, with the stream it was made on, as long as any such result lives, and a capture that
+reaches another stream through it ends in an error that torch does not recover from.
 """
 import torch
 import torch.nn.functional as F

@@ -19,14 +19,14 @@
 // What bounds them at full size is the matrix pipe together with the vector work between its products (an exponential, its
 // scaling and its rounding per score): 2 x 4096 x 16 heads x 128 without a mask runs forward at 900 TFLOP/s, forward for a
 // backward pass at 1070 and backward at 1170 TFLOP/s of the products it executes, where a library matmul of 8192^3 reaches
-// 1190.  LDS reads take 16 % of the cycles and conflicts none; reading fragments further ahead changes nothing.  Three choices
-// made that rate:
+// 1190.  LDS reads take 16 % of the cycles there and conflicts none.  Three choices made that rate:
 //   * every kernel is compiled for two waves per SIMD (256 registers): with more, hipcc keeps the sums in accumulation
 //     registers and spends hundreds of moves per tile on them (dk / dv 1173 us -> 563 us), and a single spilled register
 //     in the loop waits for the prefetch behind it (563 -> 358 us without);
 //   * 32 columns (queries, or keys) per wave where the sums fit, so a fragment from LDS feeds two products; at head_dim 256
 //     and above 16 columns with the whole row in one wave beat 32 with the row shared by two, whose scores have to meet
-//     in LDS (8 x 3136 x 784 x 256: 60 -> 42 us).  Only the sums of dq, dk / dv over 512 columns need the sharing;
+//     in LDS (8 x 3136 x 784 x 256: 60 -> 42 us), and 32 columns with the whole row spill or leave one wave
+//     per SIMD (74 - 99 us).  Only the sums of dq, dk / dv over 512 columns need the sharing;
 //   * masks stand behind uniform branches, so tiles inside the sequence pay nothing for them.
 #include "lds_dma.h"
 #include <math.h>
@@ -215,7 +215,8 @@ template <bool FINE> __device__ __forceinline__ void at_store_out(const AttnArgs
 }
 
 // Fragments are read AT_AHEAD ahead of the products that take them: an LDS read takes longer than the NT products of one
-// fragment, and left alone hipcc reads each one right in front of its use.
+// fragment, and left alone hipcc reads each one right in front of its use (one ahead in hipcc's own order: 2 x 4096 x 16 heads x
+// 128 forward 355 -> 363 us, backward 821 -> 836, 8 x 3136 x 784 x 256 41 -> 45; two or six ahead as four).
 constexpr int AT_AHEAD = 4;
 __device__ __forceinline__ void at_order() { __builtin_amdgcn_sched_barrier(0); }
 
