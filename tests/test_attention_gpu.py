@@ -175,6 +175,20 @@ def test_split_keys(D):
     run_case(1, 1500, 33, 1, 1, D, False, "none")      # dk / dv split over the queries
 
 
+@pytest.mark.parametrize("D,causal", [(24, False), (64, True), (128, False), (128, True), (256, False), (512, False), (512, True)])
+def test_grids_that_fill_the_card(D, causal):
+    """so many heads that whole tiles of rows are taken (the other tests' calls get half tiles)"""
+    run_case(26, 130, 140, 10, 10, D, causal, "both")
+
+
+def test_grids_that_fill_the_card_by_rows_or_by_splits():
+    run_case(35, 130, 140, 8, 4, 128, False, "none")
+    run_case(11, 120, 130, 6, 6, 512, False, "both")
+    run_case(1, 200, 4500, 2, 2, 512, False, "keys")
+    run_case(1, 100, 9000, 2, 1, 128, False, "none")    # long shares: whole tiles in splits
+    run_case(1, 100, 9000, 1, 1, 128, True, "keys")
+
+
 @pytest.mark.parametrize("spread,scale", [(6.0, None), (1.0, 3.0), (0.01, None), (1.0, 1e-6)])
 def test_peaked_and_flat_rows(spread, scale):
     run_case(2, 65, 140, 2, 2, 64, False, "none", scale=scale, spread=spread)

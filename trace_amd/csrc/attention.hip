@@ -922,41 +922,67 @@ static inline size_t at_align(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Splits so that about `per_cu` workgroups per CU exist, each with at least `min_iters` iterations of its loop (32 rows): the
 // partial results cost a pass over f32 copies of the output and a launch.  4 x 500 x 4 heads x 128: forward 18.9 us with at least
-// 8, 21.3 with 4, 25.9 with 2; backward 46.3 with 4, 50.0 with 8, 57.4 with 2.
+// 8, 21.3 with 4, 25.9 with 2; backward 46.3 with 4, 50.0 with 8, 57.4 with 2.  At most `per_cu` each, or a few of them would run
+// alone at the end (1 x 3136 x 784 x 512, backward: 13 key tiles in 20 shares 122 us, in 17 78 us), and no empty shares.
 static int at_splits(long long groups, int iters, int min_iters, int per_cu) {
-  if (groups <= 0 || 2 * groups > per_cu * AT_CUS) return 1;
-  long long s = (per_cu * AT_CUS + groups - 1) / groups;
+  if (groups <= 0 || iters <= 0) return 1;
+  long long s = per_cu * AT_CUS / groups;
   const long long most = iters / min_iters;
   if (s > most) s = most;
   if (s > AT_MAX_SPLITS) s = AT_MAX_SPLITS;
-  return s < 1 ? 1 : (int)s;
+  if (s <= 1) return 1;
+  const int per = ceil_div(iters, s);
+  return ceil_div(iters, per);
+}
+
+// Whether half a tile of rows serves a call better than a whole one: where whole tiles would have to be split to fill the card and
+// their shares stay short (`most` iterations), the joining of the shares costs more than half tiles, whose fragments from LDS feed
+// half the products.  Forward / backward, whole against half: 128 x 8 heads causal, 8 x 1024: 54 -> 35 us / 155 -> 95, 16 x 512: 46 ->
+// 25 / 133 -> 66; 4 x 1024: 39 -> 30 / 99 -> 89; 16 x 197 x 12 heads x 64: bwd 32 -> 29; 8 x 500 x 4 heads x 256: bwd 81 -> 62.  Longer
+// shares (1 x 4096 x 8 heads x 128: 64 iterations): 103 -> 112 / 251 -> 296; full grids (8 x 1024): 46 -> 54 / 129 -> 157.
+static bool at_short(long long groups, int iters, int min_iters, int per_cu, int most) {
+  return 2 * groups <= per_cu * AT_CUS && ceil_div(iters, at_splits(groups, iters, min_iters, per_cu)) <= most;
 }
 
 static AttnPlan at_plan(const trace_attention_desc* d) {
   AttnPlan pl;
   const int hd = d->head_dim;
   pl.D = hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
-  const int G = d->heads / d->kv_heads;
+  const int G = d->heads / d->kv_heads, uneven = d->causal ? 2 : 1;   // uneven work: more, shorter workgroups
+  const long long qh = (long long)d->heads * d->batch, kh = (long long)d->kv_heads * d->batch;
+  const int k_iters = ceil_div(d->k_rows, 32), q_iters = ceil_div(d->q_rows, 32) * G;
+  const auto q_groups = [&](int rows) { return ceil_div(d->q_rows, rows) * qh; };
+  // head_dim 512: 32 rows with four waves where 64-row tiles with their splits reach half of the CUs at most (too few keys to split):
+  // 8 x 784 rows over 196 keys, forward for a backward pass 28 -> 21 us, dq 29 -> 23; where they can be split, whole tiles are
+  // ahead (2 x 2048 x 2048 50 against 65 us)
+  const auto half512 = [&](int min_iters) {
+    return q_groups(64) * at_splits(q_groups(64), k_iters, min_iters, uneven) <= AT_CUS / 2;
+  };
+
   // few query rows: all heads of a key head on one row axis, 16 rows per workgroup (its one row group streams the keys)
   const bool small = (long long)d->q_rows * G <= 16;
   pl.pack = small ? G : 1;
   pl.units = d->heads / pl.pack;
-  pl.tile_rows = small ? 16 : pl.D <= 128 ? 128 : 64;
-  // head_dim 512, one workgroup of eight waves per CU: 128 rows with each wave on a whole row where that fills the card (4 x 4 x
-  // 2048 rows: 111 against 133 us), else 64 rows with two waves on each (8 x 784 rows over 196 keys: 22 against 28 us)
-  if (pl.D == 512 && !small && (long long)ceil_div(d->q_rows, 128) * d->heads * d->batch >= AT_CUS) pl.tile_rows = 128;
+  const int held = (small ? (pl.D <= 128 ? 5 : pl.D == 256 ? 2 : 1) : (pl.D <= 256 ? 2 : 1) * uneven);   // workgroups that a CU holds, by their LDS
+  if (small) pl.tile_rows = 16;
+  else if (pl.D <= 128) pl.tile_rows = at_short(q_groups(128), k_iters, 8, held, 16) ? 64 : 128;
+  else if (pl.D == 256) pl.tile_rows = 64;
+  // one workgroup of eight waves per CU: 128 rows with each wave on a whole row where that fills the card (4 x 4 x 2048 rows: 111
+  // against 133 us), else 64 rows with two waves on each (8 x 784 rows over 196 keys: 22 against 28 us), or half of that
+  else pl.tile_rows = q_groups(128) >= AT_CUS ? 128 : half512(8) ? 32 : 64;
   pl.tiles = ceil_div((long long)pl.pack * d->q_rows, pl.tile_rows);
-  const int uneven = d->causal ? 2 : 1;   // uneven work: more, shorter workgroups
-  const int held = small ? (pl.D <= 128 ? 5 : pl.D == 256 ? 2 : 1) : (pl.D <= 256 ? 2 : 1) * uneven;   // workgroups that a CU holds, by their LDS
-  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch, ceil_div(d->k_rows, 32), small ? 4 : 8, held);
-  const int bwd_rows = pl.D <= 256 ? 128 : 64;
+  pl.splits = at_splits((long long)pl.tiles * pl.units * d->batch, k_iters, small ? 4 : 8, held);
+
   const int per_cu = (pl.D <= 128 ? 2 : 1) * uneven;   // workgroups that a CU holds, by their LDS
-  pl.q_rows = bwd_rows;
+  pl.q_rows = pl.D <= 256 ? (at_short(q_groups(128), k_iters, 4, per_cu, 16) ? 64 : 128) : half512(4) ? 32 : 64;
   pl.q_tiles = ceil_div(d->q_rows, pl.q_rows);
-  pl.q_splits = at_splits((long long)pl.q_tiles * d->heads * d->batch, ceil_div(d->k_rows, 32), 4, per_cu);
+  pl.q_splits = at_splits(pl.q_tiles * qh, k_iters, 4, per_cu);
+  // head_dim 512: 64 keys with two waves on each row or 32 with four (8 x 784 rows over 196 keys with the reduction of the splits 35 ->
+  // 31 us; 4 x 3136 over 784, whose shares are long, backward 155 against 181)
   pl.k_rows = pl.D <= 256 ? 128 : 64;
+  if (at_short(ceil_div(d->k_rows, pl.k_rows) * kh, q_iters, 4, per_cu, pl.D <= 256 ? 16 : 8)) pl.k_rows /= 2;
   pl.k_tiles = ceil_div(d->k_rows, pl.k_rows);
-  pl.k_splits = at_splits((long long)pl.k_tiles * d->kv_heads * d->batch, ceil_div(d->q_rows, 32) * G, 4, per_cu);
+  pl.k_splits = at_splits(pl.k_tiles * kh, q_iters, 4, per_cu);
   return pl;
 }
 
@@ -1077,12 +1103,16 @@ extern "C" int trace_attention_fwd_bf16(const trace_attention_desc* d, const uin
       default: rc = at_launch_fwd<512, 1, 4, 4, 32>(a, st); break;
     }
   } else {
+    const bool whole = pl.tile_rows == 128;
     switch (pl.D) {
-      case 32: rc = at_launch_fwd<32, 2, 4, 1, 64>(a, st); break;
-      case 64: rc = at_launch_fwd<64, 2, 4, 1, 64>(a, st); break;
-      case 128: rc = at_launch_fwd<128, 2, 4, 1, 64>(a, st); break;
+      case 32: rc = whole ? at_launch_fwd<32, 2, 4, 1, 64>(a, st) : at_launch_fwd<32, 1, 4, 1, 64>(a, st); break;
+      case 64: rc = whole ? at_launch_fwd<64, 2, 4, 1, 64>(a, st) : at_launch_fwd<64, 1, 4, 1, 64>(a, st); break;
+      case 128: rc = whole ? at_launch_fwd<128, 2, 4, 1, 64>(a, st) : at_launch_fwd<128, 1, 4, 1, 64>(a, st); break;
       case 256: rc = at_launch_fwd<256, 1, 4, 1, 32>(a, st); break;
-      default: rc = pl.tile_rows == 128 ? at_launch_fwd<512, 1, 8, 1, 32>(a, st) : at_launch_fwd<512, 1, 8, 2, 32>(a, st); break;
+      default:
+        rc = whole ? at_launch_fwd<512, 1, 8, 1, 32>(a, st)
+             : pl.tile_rows == 64 ? at_launch_fwd<512, 1, 8, 2, 32>(a, st) : at_launch_fwd<512, 1, 4, 2, 32>(a, st);
+        break;
     }
   }
   if (rc) return rc;
@@ -1151,12 +1181,13 @@ extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uin
   if (d->q_rows > 0) {
     a.tiles = pl.q_tiles;
     a.splits = pl.q_splits;
+    const bool whole = pl.q_rows == (pl.D <= 256 ? 128 : 64);
     switch (pl.D) {
-      case 32: rc = at_launch_q<32, 2, 4, 1>(a, st); break;
-      case 64: rc = at_launch_q<64, 2, 4, 1>(a, st); break;
-      case 128: rc = at_launch_q<128, 2, 4, 1>(a, st); break;
-      case 256: rc = at_launch_q<256, 1, 8, 1>(a, st); break;
-      default: rc = at_launch_q<512, 1, 8, 2>(a, st); break;
+      case 32: rc = whole ? at_launch_q<32, 2, 4, 1>(a, st) : at_launch_q<32, 1, 4, 1>(a, st); break;
+      case 64: rc = whole ? at_launch_q<64, 2, 4, 1>(a, st) : at_launch_q<64, 1, 4, 1>(a, st); break;
+      case 128: rc = whole ? at_launch_q<128, 2, 4, 1>(a, st) : at_launch_q<128, 1, 4, 1>(a, st); break;
+      case 256: rc = whole ? at_launch_q<256, 1, 8, 1>(a, st) : at_launch_q<256, 1, 4, 1>(a, st); break;
+      default: rc = whole ? at_launch_q<512, 1, 8, 2>(a, st) : at_launch_q<512, 1, 4, 2>(a, st); break;
     }
     if (rc) return rc;
     if (int e = check_launch("attention backward (dq)")) return e;
@@ -1169,12 +1200,13 @@ extern "C" int trace_attention_bwd_bf16(const trace_attention_desc* d, const uin
   if (d->k_rows > 0) {
     a.tiles = pl.k_tiles;
     a.splits = pl.k_splits;
+    const bool whole = pl.k_rows == (pl.D <= 256 ? 128 : 64);
     switch (pl.D) {
-      case 32: rc = at_launch_kv<32, 2, 4, 1>(a, st); break;
-      case 64: rc = at_launch_kv<64, 2, 4, 1>(a, st); break;
-      case 128: rc = at_launch_kv<128, 2, 4, 1>(a, st); break;
-      case 256: rc = at_launch_kv<256, 1, 8, 1>(a, st); break;
-      default: rc = at_launch_kv<512, 1, 8, 2>(a, st); break;
+      case 32: rc = whole ? at_launch_kv<32, 2, 4, 1>(a, st) : at_launch_kv<32, 1, 4, 1>(a, st); break;
+      case 64: rc = whole ? at_launch_kv<64, 2, 4, 1>(a, st) : at_launch_kv<64, 1, 4, 1>(a, st); break;
+      case 128: rc = whole ? at_launch_kv<128, 2, 4, 1>(a, st) : at_launch_kv<128, 1, 4, 1>(a, st); break;
+      case 256: rc = whole ? at_launch_kv<256, 1, 8, 1>(a, st) : at_launch_kv<256, 1, 4, 1>(a, st); break;
+      default: rc = whole ? at_launch_kv<512, 1, 8, 2>(a, st) : at_launch_kv<512, 1, 8, 4>(a, st); break;
     }
     if (rc) return rc;
     if (int e = check_launch("attention backward (dk, dv)")) return e;
