@@ -194,6 +194,19 @@ def test_peaked_and_flat_rows(spread, scale):
     run_case(2, 65, 140, 2, 2, 64, False, "none", scale=scale, spread=spread)
 
 
+@pytest.mark.parametrize("D", [8, 16, 32])
+def test_dq_of_few_columns(D):
+    """dq carries no more than its own rounding: at most u |dq| each, so u / sqrt(3) in the root mean square if spread evenly (a
+    rounded dS would add as much again, and more the fewer the columns, because its rows sum to zero)"""
+    from trace_amd import ops
+    q, k, v, do = make(2, 300, 400, 4, 2, D, 21)
+    ref, _, _ = reference(q, k, v, do, D ** -0.5, False, [(300, 400)] * 2)
+    q, k, v, do = (t.to(DEV) for t in (q, k, v, do))
+    dq, _, _ = ops.attention_backward(do, q, k, v, *ops.attention(q, k, v, for_backward=True))
+    want = ref["dq"][0]
+    assert float((dq.double().cpu() - want).norm() / want.norm()) < U / 3 ** 0.5
+
+
 def test_no_keys_no_rows():
     from trace_amd import ops
     q, k, v, do = (t.to(DEV) for t in make(2, 5, 0, 2, 1, 64, 3))

@@ -548,11 +548,16 @@ template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_few_ker
 // second one starts from -delta instead of zero.  dS is rounded to bf16 for the product, as P is in the forward kernel.  dq and
 // dk / dv each form P and dS for themselves: seven products instead of the five of one pass, whose dq (or dk, dv) would have to
 // be added up by atomics in whatever order workgroups come.  2 x 4096 x 16 heads x 128, causal: 221 us, dk / dv 299 us.
+// The rows of dS sum to zero, so dq only has what the keys differ by, but the rounding of dS goes with all of a key: with few
+// columns the weighted mean of the keys is a good part of them (|k|^2 of D + 4 against D + 1 for unit normal q, k), and dq is
+// less exact than its own rounding explains.  Up to 32 columns a second product therefore adds what that rounding lost
+// (relative error at 8 columns 2.56e-3 -> 1.65e-3, at 16 2.48e-3 -> 1.67e-3; 4 x 2048 x 16 heads x 32: backward 170 -> 195 us).
 // ---------------------------------------------------------------------------------------------------------------
 template <int D, int NT, int NW, int DW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p) {
   constexpr int BN = 32, TR = NW / DW * NT * 16, KC = D / 32 / DW, DT = D / 16 / DW;
   constexpr int TILE = BN * D * 2;
+  constexpr bool FINE = D <= 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wd = wave % DW, wr = wave / DW;
@@ -667,7 +672,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
     AtTrAhead<D, DT, 1> ka;
     ka.start(smem, tr_at + stage);
     const bool mask = key0 + BN > wmin;
-    at_s8 ds[NT];
+    at_s8 ds[NT], dl[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -686,12 +691,20 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
             if (key0 + st * 16 + 4 * g + r >= lim[nt]) s[st][nt][r] = 0.f;
     }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) ds[nt] = at_pack8(s[0][nt] * dp[0][nt], s[1][nt] * dp[1][nt]);
+    for (int nt = 0; nt < NT; ++nt) {
+      const at_f4 lo = s[0][nt] * dp[0][nt], hi = s[1][nt] * dp[1][nt];
+      ds[nt] = at_pack8(lo, hi);
+      if constexpr (FINE) dl[nt] = at_lost8(lo, hi, ds[nt]);
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const at_s8 a = ka.take(smem, tr_at + stage, dt);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, ds[nt], acc[dt][nt]);
+      if constexpr (FINE) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[dt][nt] = at_mfma(a, dl[nt], acc[dt][nt]);
+      }
       at_order();
     }
   }
