@@ -35,6 +35,7 @@ struct GnArgs {
   int slab;             // groups per workgroup of the one-pass form
   int pow2;             // its columns, and those of a group, are powers of two of whole accesses
   int rows, chunks;     // two-pass: rows per chunk
+  int nt;               // two-pass: results are stored past the caches
 };
 
 // V elements of T as loaded: bf16 as 32-bit words of two (one element alone: itself), f32 as they are
@@ -454,7 +455,23 @@ __device__ __forceinline__ GnMom gn_merge(const GnMom& a, const GnMom& b) {
   return {n, a.mean + d * w, a.m2 + b.m2 + d * d * a.n * w};
 }
 
-constexpr int GN_U = 8;   // rows a thread loads before it uses them
+// rows a thread loads before it uses them; in the backward kernels, where a row is two loads, half as many (8 x 25088 x 256
+// without an activation: backward 109 -> 103 us; 8 rows leave registers for three waves per SIMD only)
+constexpr int GN_U = 8, GN_UB = 4;
+
+// The result of the last pass.  Maps beyond GN_NT_BYTES are stored past the caches: written lines would push out what the pass
+// still has to read there (8 x 25088 x 256, SiLU: forward 77 -> 69 us, backward 123 -> 112; with the copies that write x and dy and read the
+// results 315 -> 306).  Smaller maps stay for whoever reads them next (49 MB: 182 us in that chain, 186 past the caches).
+constexpr long long GN_NT_BYTES = 64ll << 20;
+template <typename Raw> __device__ __forceinline__ void gn_store(void* at, const Raw& v, int nt) {
+  if (nt) {
+    asm volatile("");   // else the compiler makes one plain store of the two
+    __builtin_nontemporal_store(v, static_cast<Raw*>(at));
+    asm volatile("");
+  } else {
+    *static_cast<Raw*>(at) = v;
+  }
+}
 
 template <typename T, int V>
 __global__ __launch_bounds__(GN_CT) void gn_stats_kernel(const GnArgs p) {
@@ -624,7 +641,7 @@ __global__ __launch_bounds__(GN_CT) void gn_apply_kernel(const GnArgs p) {
 #pragma unroll
           for (int v = 0; v < V; ++v) f[v] = (f[v] - mean[v]) * ga[v] + be[v];
           gn_act<V>(f, p.act);
-          *reinterpret_cast<Raw*>(y + (long long)(row + i * RP) * p.C) = gn_pack<T, V>(f);
+          gn_store<Raw>(y + (long long)(row + i * RP) * p.C, gn_pack<T, V>(f), p.nt);
           gn_row_done();
         }
     }
@@ -658,16 +675,16 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_sums_kernel(const GnArgs p) {
         be[v] = p.beta ? p.beta[c] : 0.f;
         a[v] = b[v] = 0.f;
       }
-      for (int row = row0 + rr; row < row1; row += GN_U * RP) {
-        Raw rx[GN_U], rd[GN_U];
+      for (int row = row0 + rr; row < row1; row += GN_UB * RP) {
+        Raw rx[GN_UB], rd[GN_UB];
 #pragma unroll
-        for (int i = 0; i < GN_U; ++i)
+        for (int i = 0; i < GN_UB; ++i)
           if (row + i * RP < row1) {
             rx[i] = *reinterpret_cast<const Raw*>(x + (long long)(row + i * RP) * p.C);
             rd[i] = *reinterpret_cast<const Raw*>(dy + (long long)(row + i * RP) * p.C);
           }
 #pragma unroll
-        for (int i = 0; i < GN_U; ++i)
+        for (int i = 0; i < GN_UB; ++i)
           if (row + i * RP < row1) {
             float f[V], d[V], z[V];
             gn_unpack<T, V>(rx[i], f);
@@ -787,16 +804,16 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_apply_kernel(const GnArgs p) {
       ga[v] = p.gamma ? p.gamma[c] : 1.f;
       be[v] = p.beta ? p.beta[c] : 0.f;
     }
-    for (int row = row0 + rr; row < row1; row += GN_U * RP) {
-      Raw rx[GN_U], rd[GN_U];
+    for (int row = row0 + rr; row < row1; row += GN_UB * RP) {
+      Raw rx[GN_UB], rd[GN_UB];
 #pragma unroll
-      for (int i = 0; i < GN_U; ++i)
+      for (int i = 0; i < GN_UB; ++i)
         if (row + i * RP < row1) {
           rx[i] = *reinterpret_cast<const Raw*>(x + (long long)(row + i * RP) * p.C);
           rd[i] = *reinterpret_cast<const Raw*>(dy + (long long)(row + i * RP) * p.C);
         }
 #pragma unroll
-      for (int i = 0; i < GN_U; ++i)
+      for (int i = 0; i < GN_UB; ++i)
         if (row + i * RP < row1) {
           float f[V], d[V], z[V];
           gn_unpack<T, V>(rx[i], f);
@@ -809,7 +826,7 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_apply_kernel(const GnArgs p) {
           gn_dact<V>(z, d, p.act);
 #pragma unroll
           for (int v = 0; v < V; ++v) d[v] = (d[v] * ga[v] - a[v] - f[v] * b[v]) * rstd[v];
-          *reinterpret_cast<Raw*>(dx + (long long)(row + i * RP) * p.C) = gn_pack<T, V>(d);
+          gn_store<Raw>(dx + (long long)(row + i * RP) * p.C, gn_pack<T, V>(d), p.nt);
           gn_row_done();
         }
     }
@@ -943,6 +960,7 @@ static int gn_call(bool backward, const T* x, const T* dy, int N, long long P, i
   }
   a.rows = pl.rows;
   a.chunks = pl.chunks;
+  a.nt = (long long)N * P * C * sizeof(T) > GN_NT_BYTES;
   if constexpr (std::is_same<T, float>::value) {
     switch (pl.V) {
       case 4: return gn_run<T, 4>(a, pl, backward, st);
