@@ -295,6 +295,22 @@ def test_autograd_only_where_needed_and_differences():
     assert torch.equal(gv, lv.grad)
 
 
+def test_second_derivatives_are_refused():
+    """a recorded backward pass gives the same gradients, and an error only where it is differentiated itself"""
+    from trace_amd import autograd as tag
+    q, k, v, do = (t.to(DEV) for t in make(1, 20, 30, 2, 2, 32, 4))
+    w = torch.ones(32, device=DEV)
+    for f in (lambda x: tag.attention(x, k, v), lambda x: tag.group_norm_act(x, 8, w, None, 1e-5, "silu"),
+              lambda x: tag.dropout_act(x, 0.5, 1, 2, "leaky")):
+        x = q.clone().requires_grad_(True)
+        (want,) = torch.autograd.grad(f(x), x, do)
+        g = do.clone().requires_grad_(True)
+        (got,) = torch.autograd.grad(f(x), x, g, create_graph=True)
+        assert torch.equal(got, want) and got.requires_grad and not want.requires_grad
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            got.float().sum().backward()
+
+
 def test_graph_replays_and_streams():
     from trace_amd import autograd as tag, ops
     q, k, v, do = (t.to(DEV) for t in make(2, 100, 600, 2, 2, 64, 11))

@@ -22,6 +22,8 @@ Capturing a backward pass into a graph: let go of every result of an eager pass 
 leaves).  torch keeps a leaf's gradient node, with the stream it was made on, as long as any such result lives, and a capture that
 reaches another stream through it ends in an error that torch does not recover from.
 """
+import functools
+
 import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
@@ -149,6 +151,21 @@ def gemm_nt(x, w, bias=None, relu=False):
     return _GemmNT.apply(x, w, bias, bool(relu))
 
 
+def _once(backward):
+    """once_differentiable, which only a backward pass that is itself recorded (create_graph) has to pay for: its no_grad block
+    costs as much host time as two launches."""
+    recorded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
+def _as(t, dtype):
+    return t if t.dtype == dtype else t.to(dtype)
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, causal, q_len, kv_len):
@@ -158,10 +175,10 @@ class _Attention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gout):
         q, k, v, out, lse, rest, q_len, kv_len = ctx.saved_tensors
-        grads = ops.attention_backward(gout.to(torch.bfloat16), q, k, v, out, lse, rest, *ctx.cfg, q_len, kv_len)
+        grads = ops.attention_backward(_as(gout, torch.bfloat16), q, k, v, out, lse, rest, *ctx.cfg, q_len, kv_len)
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,) * 4
 
 
@@ -183,13 +200,13 @@ class _GroupNormAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gy):
         x, stats, gamma, beta = ctx.saved_tensors
         groups, act = ctx.cfg
         need = ctx.needs_input_grad
-        dx, dg, db = ops.group_norm_act_backward(gy.to(x.dtype), x, stats, groups, gamma, beta, act, param_grads=need[2] or need[3])
-        return (dx if need[0] else None, None, dg.to(gamma.dtype) if need[2] else None, db.to(beta.dtype) if need[3] else None,
+        dx, dg, db = ops.group_norm_act_backward(_as(gy, x.dtype), x, stats, groups, gamma, beta, act, param_grads=need[2] or need[3])
+        return (dx if need[0] else None, None, _as(dg, gamma.dtype) if need[2] else None, _as(db, beta.dtype) if need[3] else None,
                 None, None)
 
 
@@ -208,11 +225,11 @@ class _DropoutAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gy):
         x, step = ctx.saved_tensors
         p, seed, offset, act, dt = ctx.cfg
-        return (ops.dropout_act_backward(gy.to(dt), x, p, seed, offset, act, step),) + (None,) * 5
+        return (ops.dropout_act_backward(_as(gy, dt), x, p, seed, offset, act, step),) + (None,) * 5
 
 
 def dropout_act(x, p, seed, offset=0, act=None, step=None, training=True):

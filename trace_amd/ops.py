@@ -958,6 +958,10 @@ def _scratch(nbytes, dev):
     return torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
 
 
+def _empty_as(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _attn_operand(t, name):
     """(B, N, heads, D) bf16 on the GPU as the kernels take it: last dimension contiguous, rows 16-byte aligned, the other
     strides multiples of 8 elements (any order, 0 where a dimension is broadcast).  Other layouts are copied."""
@@ -1046,13 +1050,12 @@ def attention_backward(dout, q, k, v, out, lse, rest, scale=None, causal=False, 
     d = _attn_desc(q, k, v, scale, causal, q_len, kv_len)
     if lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (B, H, Nq) or lse.device != dev:
         raise RuntimeError("attention_backward: lse must be the (batch, heads, rows) float32 tensor of the forward call")
+    shape = q.shape
     for t, n in ((out, "out"), (rest, "rest"), (dout, "dout")):
-        if t.shape != q.shape or t.device != dev or t.dtype != torch.bfloat16 or not (t.is_contiguous() or t is dout):
+        if t.shape != shape or t.device != dev or t.dtype != torch.bfloat16 or not (t is dout or t.is_contiguous()):
             raise RuntimeError("attention_backward: %s %s %s does not match q %s" % (n, tuple(t.shape), t.dtype, tuple(q.shape)))
     d.stride_do = _attn_strides(dout)
-    dq = torch.empty((B, Nq, H, D), dtype=torch.bfloat16, device=dev)
-    dkv = torch.empty((2,) + tuple(k.shape), dtype=torch.bfloat16, device=dev)
-    dk, dv = dkv.unbind(0)
+    dq, dk, dv = torch.empty_like(out), _empty_as(k), _empty_as(v)
     lib = L.lib()
     n = lib.trace_attention_bwd_workspace_bytes(d)
     ws = _scratch(n, dev)
@@ -1130,7 +1133,7 @@ def group_norm_act_backward(dy, x, stats, groups, gamma=None, beta=None, act=Non
     if stats.device != dev or stats.dtype != torch.float32 or stats.shape != (N, groups, 2) or not stats.is_contiguous():
         raise RuntimeError("group_norm_act_backward: stats must be the (N, groups, 2) float32 tensor of the forward call")
     dx = torch.empty_like(x)
-    dg, db = torch.empty((2, C), dtype=torch.float32, device=dev).unbind(0) if param_grads else (None, None)
+    dg, db = (stats.new_empty((C,)), stats.new_empty((C,))) if param_grads else (None, None)
     lib = L.lib()
     n = _gn_workspace(N, P, C, groups, 1)
     ws = _scratch(n, dev)
