@@ -166,7 +166,7 @@ class NonLocal3d(nn.Module):
     """mmcv.cnn.NonLocal3d (mmcv 1.x `_NonLocalNd`), the configuration TRACE uses
     (i3d_nl_dot_product_...py:15-19: sub_sample=True, use_scale=False,
     mode='dot_product', BN on conv_out).  Source not vendored in the reference:
-    restated from mmcv's published behaviour (SURVEY.md A.2, parity unpinned).
+    restated from mmcv's published behaviour (parity unpinned).
     mode='embedded_gaussian' (mmcv's default) is softmax attention of every position over the (pooled) positions, with
     use_scale divided by sqrt(inter_channels); it runs on ops.attention and needs inter_channels % 8 == 0, <= 512."""
 
