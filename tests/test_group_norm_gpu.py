@@ -332,6 +332,24 @@ def test_nonlocal_embedded_gaussian(sub, use_scale):
         assert rel(p.grad, ref[n]) < (5e-2 if n.startswith(("phi.", "g.", "theta.")) else 2e-2), (n, rel(p.grad, ref[n]))
 
 
+def test_nonlocal_embedded_gaussian_keeps_the_f32_residual_stream():
+    from trace_amd.resnet3d import NonLocal3d
+    torch.manual_seed(6)
+    nl = NonLocal3d(128, sub_sample=True, use_scale=True, mode='embedded_gaussian', norm_cfg=dict(type='BN3d')).eval().to(DEV)
+    with torch.no_grad():
+        nl.conv_out.bn.weight.fill_(1.0)
+        x32 = torch.randn((2, 2, 6, 6, 128), device=DEV) * 4
+        x = x32.bfloat16()
+        plain = nl.run(x)
+        assert not hasattr(plain, "_res32")
+        x._res32 = x32
+        out = nl.run(x)
+        assert out.dtype == torch.bfloat16 and torch.equal(out._res32.bfloat16(), out)
+        # plain is x + y rounded to bf16, out x32 + y; x itself is half a bf16 step from x32
+        step = 2.0 ** -8 * (plain.float().abs() + x32.abs()) + 1e-5
+        assert bool(((out._res32 - x32) - (plain.float() - x.float())).abs().le(step).all())
+
+
 def test_refusals():
     from trace_amd import ops
     x = torch.zeros((2, 10, 16), device=DEV)

@@ -262,6 +262,13 @@ class NonLocal3d(nn.Module):
                 theta, pg = tpg[..., :c], tpg[..., c:]
             phi, g = pg[..., :c], pg[..., c:]
             y = ops.attention(theta, phi, g, self._scale())
+            x32 = getattr(x, "_res32", None)
+            if x32 is not None and not self.conv_out.with_gn:   # f32 residual stream, as below
+                w_out, b_out = self.conv_out.packed()
+                o32, o16 = ops.gemm_nt(y.view(N * nq, c), w_out, bias=b_out, residual=x32.view(N * nq, C), out_f32=True, out2="none")
+                out = o16.view(N, T, H, W, C)
+                out._res32 = o32.view(N, T, H, W, C)
+                return out
             return self.conv_out.run(y.view(N, T, H, W, c), residual=x, relu=False)
         if self.sub_sample and c % 64 == 0:
             # theta|phi|g in one launch, then ONE kernel pools phi / g and lays them out for the products
