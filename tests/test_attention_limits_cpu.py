@@ -26,3 +26,23 @@ def test_rows_whose_tiles_pass_32_bits_are_refused(kw):
     # no pointers but the call is refused for its rows, in front of anything else
     assert l.trace_attention_fwd_bf16(d, *[None] * 7, 0, None) != 0 and b"too many rows" in l.trace_last_error()
     assert l.trace_attention_bwd_bf16(d, *[None] * 11, 0, None) != 0 and b"too many rows" in l.trace_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(batch=1 << 10, heads=1 << 10, q_rows=(1 << 11) - 2), dict(batch=1 << 10, heads=1 << 10, kv_heads=1 << 10, k_rows=1 << 11),
+                                dict(batch=1 << 20, heads=1 << 12, kv_heads=4)])
+def test_grids_past_32_bits_are_refused(kw):
+    from trace_amd import _lib as L
+    d = desc(**kw)
+    assert L.lib().trace_attention_fwd_bf16(d, *[None] * 7, 0, None) != 0 and b"too many rows" in L.lib().trace_last_error()
+    assert L.lib().trace_attention_bwd_bf16(d, *[None] * 11, 0, None) != 0 and b"too many rows" in L.lib().trace_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(batch=128, heads=64, kv_heads=8, q_rows=1, k_rows=262144, head_dim=128), dict(heads=8, kv_heads=1, k_rows=1 << 30),
+                                dict(batch=1 << 12, heads=1 << 9, q_rows=1, k_rows=1 << 16)])
+def test_query_heads_times_key_rows_is_no_limit(kw):
+    """the call passes the check of its sizes: the next thing that is wrong with it, null pointers, is what it is refused for"""
+    from trace_amd import _lib as L
+    d = desc(**kw)
+    assert L.lib().trace_attention_bwd_workspace_bytes(d) > 0
+    assert L.lib().trace_attention_fwd_bf16(d, *[None] * 7, 0, None) != 0 and b"null pointer" in L.lib().trace_last_error()
+    assert L.lib().trace_attention_bwd_bf16(d, *[None] * 11, 0, None) != 0 and b"null pointer" in L.lib().trace_last_error()

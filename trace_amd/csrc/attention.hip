@@ -1011,8 +1011,10 @@ static int at_check(const trace_attention_desc* d, const char* what) {
   TRACE_REQUIRE(d->scale > 0.f && d->scale <= 3.0e38f, "%s: scale must be positive and finite", what);
   // rows are counted in 32 bits to the end of the last tile, and a causal mask adds q_rows to k_rows
   TRACE_REQUIRE(d->q_rows <= AT_MAX_ROWS && d->k_rows <= AT_MAX_ROWS, "%s: too many rows (at most 2^30)", what);
-  // tiles x heads x batch are grid indices and rows x heads of a packed call row indices
-  TRACE_REQUIRE((long long)d->batch * d->heads * ((long long)d->q_rows + d->k_rows + 2) < (1ll << 31) - 1, "%s: too many rows", what);
+  // tiles x heads x batch are grid indices, of query heads over query rows (rows x heads of a packed call are row indices too) and
+  // of key heads over key rows
+  const long long qr = (long long)d->batch * d->heads * (d->q_rows + 2), kr = (long long)d->batch * d->kv_heads * (d->k_rows + 2);
+  TRACE_REQUIRE(qr < (1ll << 31) - 1 && kr < (1ll << 31) - 1, "%s: too many rows (batch x heads x rows of queries or keys)", what);
   for (int i = 0; i < 3; ++i)
     TRACE_REQUIRE(((d->stride_q[i] | d->stride_k[i] | d->stride_v[i]) & 7) == 0, "%s: strides must be multiples of 8 elements", what);
   for (long long st : {d->stride_q[1], d->stride_k[1], d->stride_v[1], d->stride_do[1]})   // 64-row tiles: 32-bit byte offsets
