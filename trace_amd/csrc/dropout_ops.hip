@@ -64,17 +64,20 @@ __global__ __launch_bounds__(256) void dropout_act_kernel(const DropArgs p) {
   const uint64_t off = p.offset + (p.step ? (uint64_t)*p.step : 0);
   const long long whole = p.n >> 3, b0 = (long long)blockIdx.x * (DROP_U * 256) + threadIdx.x;
   const bool need_x = !BWD || p.act;
-  const float low = (p.act & TRACE_EPI_RELU) ? 0.f : (p.act & TRACE_EPI_LEAKY) ? 0.1f : 1.f;
+  const bool relu = p.act & TRACE_EPI_RELU;
   const DropVec<T>*xp = static_cast<const DropVec<T>*>(p.x), *gp = static_cast<const DropVec<T>*>(p.dy);
   auto one = [&](float x, float g, uint32_t piece) {
     float v;
+    bool neg;
     if (BWD) {
       v = g * p.scale;
-      if (p.act && !(x > 0.f)) v *= low;
+      neg = p.act && !(x > 0.f);
     } else {
       v = x * p.scale;
-      if (p.act) v = v < 0.f ? v * low : v;   // NaN stays
+      neg = p.act && v < 0.f;   // NaN stays
     }
+    // relu selects: the scale may have made v infinite, and 0 times that is no zero
+    if (neg) v = relu ? 0.f : v * 0.1f;
     return piece < p.threshold ? 0.f : v;
   };
   DropVec<T> xv[DROP_U], gv[DROP_U];
