@@ -582,7 +582,8 @@ int trace_attention_bwd_bf16(const trace_attention_desc* desc, const uint16_t* q
 /* Group normalisation + activation over channels-last maps x (N, P, C), P = product of the positions, contiguous:
  *   z = (x - mean) / sqrt(var + eps) * gamma + beta with the mean / biased variance of each sample's groups of C / G
  *   channels, y = act(z); act = 0 | TRACE_EPI_RELU | TRACE_EPI_LEAKY | TRACE_EPI_SILU.  gamma / beta (C) f32, NULL = 1 / 0.
- *   stats (N, G, 2) f32: mean and 1 / sqrt(var + eps), written by the forward call, read by the backward one.
+ *   stats (N, G, 2) f32: mean and 1 / sqrt(var + eps), written by the forward call, read by the backward one (of samples without positions: 0 and
+ *   1 / sqrt(eps)).
  *   backward: dx like x, dgamma / dbeta (C) f32 (each may be NULL).
  * workspace: trace_group_norm_workspace_bytes(N, P, C, G, backward) bytes, 256-aligned.  Sums in f32 in a fixed order. */
 size_t trace_group_norm_workspace_bytes(int N, long long P, int C, int G, int backward);

@@ -758,6 +758,12 @@ __global__ __launch_bounds__(GN_CT) void gn_bwd_merge_kernel(const GnArgs p) {
   }
 }
 
+// statistics of samples without positions: mean 0, variance 0
+__global__ __launch_bounds__(256) void gn_empty_stats_kernel(const GnArgs p) {
+  const int i = blockIdx.x * 256 + threadIdx.x;   // N G stays below 2^30: gn_check
+  if (i < p.N * p.G) *reinterpret_cast<float2*>(p.stats + 2ll * i) = make_float2(0.f, 1.f / sqrtf(p.eps));
+}
+
 // dgamma / dbeta of channel c from the samples' sums, in sample order
 __device__ __forceinline__ void gn_param_grad(const GnArgs& p, int c) {
   if (c >= p.C) return;
@@ -940,6 +946,7 @@ static int gn_call(bool backward, const T* x, const T* dy, int N, long long P, i
   a.act = act;
   a.eps = eps;
   if (N == 0 || P == 0) {   // no elements: the parameters' gradients are zero
+    if (!backward && N > 0 && stats) gn_empty_stats_kernel<<<ceil_div((long long)N * G, 256), 256, 0, st>>>(a);
     a.N = 0;
     if (backward && (dgamma || dbeta)) gn_param_grad_kernel<<<ceil_div(C, 256), 256, 0, st>>>(a);
     return check_launch(what);
