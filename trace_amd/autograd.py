@@ -129,6 +129,9 @@ class _GemmNT(torch.autograd.Function):
     def backward(ctx, gy):
         xb, wb, y = ctx.saved_tensors
         relu, wdt, xdt = ctx.cfg
+        if gy.shape[0] == 0:      # no rows: sums over nothing
+            grads = (xb.to(xdt), wb.new_zeros(wb.shape, dtype=wdt), wb.new_zeros(wb.shape[:1], dtype=torch.float32))
+            return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,)
         gy = gy.to(torch.bfloat16)
         if relu:
             gy = gy * (y > 0)
