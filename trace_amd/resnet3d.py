@@ -98,6 +98,18 @@ class ConvModule(nn.Module):
         return ops.conv3d(x, w, b, c.kernel_size, c.stride, c.padding, c.dilation, residual=residual, relu=relu,
                           pool_t2=pool_t2)
 
+    def run_f32(self, x, identity, relu):
+        """GroupNorm module at the end of a block whose residual stream is f32: identity (f32) + the normalised convolution, whose
+        output is not rounded in between -> the bf16 rounding, with the f32 sum as `_res32`."""
+        w, b = self.packed()
+        c = self.conv
+        y = self._group_norm(ops.conv3d(x, w, b, c.kernel_size, c.stride, c.padding, c.dilation, out_f32=True), False)
+        y = y + identity
+        y = torch.relu_(y) if relu else y
+        out = y.to(torch.bfloat16)
+        out._res32 = y
+        return out
+
     def _group_norm(self, y, relu):
         gn = self.gn
         return ops.group_norm_act(y, gn.num_groups, gn.weight.detach().float(), gn.bias.detach().float(), gn.eps,
@@ -263,7 +275,9 @@ class NonLocal3d(nn.Module):
             phi, g = pg[..., :c], pg[..., c:]
             y = ops.attention(theta, phi, g, self._scale())
             x32 = getattr(x, "_res32", None)
-            if x32 is not None and not self.conv_out.with_gn:   # f32 residual stream, as below
+            if x32 is not None and self.conv_out.with_gn:
+                return self.conv_out.run_f32(y.view(N, T, H, W, c), x32, False)
+            if x32 is not None:      # f32 residual stream, as below
                 w_out, b_out = self.conv_out.packed()
                 o32, o16 = ops.gemm_nt(y.view(N * nq, c), w_out, bias=b_out, residual=x32.view(N * nq, C), out_f32=True, out2="none")
                 out = o16.view(N, T, H, W, C)
@@ -311,6 +325,8 @@ class NonLocal3d(nn.Module):
         # pairwise = theta^T phi / N_kv (dot_product: no softmax); y = pairwise g
         pw_full = ops.gemm_nt(theta, phi, alpha=1.0 / nkv)
         y = ops.gemm_nt(pw_full, gT)
+        if self.conv_out.with_gn and getattr(x, "_res32", None) is not None:
+            return self.conv_out.run_f32(y.view(N, T, H, W, c), x._res32, False)
         return self.conv_out.run(y.view(N, T, H, W, c), residual=x, relu=False)  # x + conv_out(y)
 
 
@@ -362,7 +378,7 @@ class Bottleneck3d(nn.Module):
         f32 twin travels as `out._res32`.  Only conv OPERANDS are rounded to bf16 then, never the running sum."""
         ds = self.downsample
         gn = self.conv3.with_gn or (ds is not None and ds.with_gn)   # nothing of a GroupNorm folds into a GEMM
-        f32 = self.res_f32 and not pool_t2 and not gn
+        f32 = self.res_f32 and not pool_t2
         fusable = (self.fuse_downsample and ds is not None and not gn and tuple(ds.conv.stride) == (1, 1, 1) and tuple(ds.conv.kernel_size) == (1, 1, 1)
                    and x.shape[-1] % 64 == 0 and self.conv3.conv.in_channels % 64 == 0 and not pool_t2)
         if fusable:
@@ -383,9 +399,13 @@ class Bottleneck3d(nn.Module):
                 c = ds.conv
                 w, b = ds.packed()
                 identity = ops.conv3d(x, w, b, c.kernel_size, c.stride, c.padding, c.dilation, out_f32=True)
+                identity = ds._group_norm(identity, False) if ds.with_gn else identity
             else:
                 identity = x32 if x32 is not None else x.float()
             h = self.conv2.run(self.conv1.run(x))
+            if gn:
+                out = self.conv3.run_f32(h, identity, True)
+                return self.non_local_block.run(out) if self.non_local else out
             w3, b3 = self.conv3.packed()
             N_, T_, H_, W_, _ = h.shape
             res = ops.gemm_nt(h.view(-1, h.shape[-1]), w3, bias=b3, residual=identity.reshape(-1, w3.shape[0]), relu=True,
