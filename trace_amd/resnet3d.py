@@ -22,7 +22,7 @@ from torch.nn.modules.utils import _ntuple, _triple
 from . import ops
 
 
-# bumped whenever folded weights are dropped (device move, state-dict load, BN recalibration): captured
+# bumped whenever folded weights are dropped (device move, state-dict load, BN recalibration, training): captured
 # graphs hold pointers into the packed tensors and are re-captured when the epoch has moved on
 _PACK_EPOCH = [0]
 
@@ -75,6 +75,17 @@ class ConvModule(nn.Module):
             self._packed = (wp, shift.contiguous(), _PACK_EPOCH[0])
         return self._packed[:2]
 
+    def _drop_folded(self):
+        """The parameters are about to be trained: what `run` (and graphs captured of it) folded from them is stale from here on."""
+        if self._packed is not None:
+            self._packed = None
+            _PACK_EPOCH[0] += 1
+
+    def train(self, mode=True):
+        if mode:      # also for captured training steps, whose replays run no Python
+            self._drop_folded()
+        return super().train(mode)
+
     def forward(self, x):
         """Plain torch path (NCTHW f32, autograd-capable): used for training-side work and for
         calibrating synthetic BN statistics; the inference hot path is `run`."""
@@ -122,6 +133,7 @@ class ConvModule(nn.Module):
         GroupNorm: the raw convolution, then the normalisation with its activation as one operator (ops.group_norm_act).
         Gradients reach conv.weight, conv.bias, the norm's weight and bias and x."""
         from . import autograd as tag
+        self._drop_folded()
         w = self.conv.weight.float()
         cout = w.shape[0]
         if self.with_gn:
