@@ -764,6 +764,53 @@ __global__ __launch_bounds__(256) void gn_empty_stats_kernel(const GnArgs p) {
   if (i < p.N * p.G) *reinterpret_cast<float2*>(p.stats + 2ll * i) = make_float2(0.f, 1.f / sqrtf(p.eps));
 }
 
+// The same in two launches where a thread of the merge above would add more than GN_LIST chunks one after the other, which few
+// threads do if the groups are wide (one workgroup, a thread per channel, for a single group of 256 channels and more): tiles of
+// eight channels with 32 lists of chunks each, then the groups.  Backward, one launch -> two: 1 x 25088 x 2048, 32 groups 129 ->
+// 104 us, one group 1188 -> 108 us (lists of 392 and 1568); 4 x 25088 x 256, 4 groups 69 -> 62 (98); short lists: 8 x 25088 x 256,
+// 32 groups 95 -> 98 (7), 1 x 6000 x 128, 8 groups 22 -> 32 (6).  A parameter's gradient, too, is then no row of up to 2048 terms.
+constexpr int GN_LIST = 64;
+__global__ __launch_bounds__(GN_CT) void gn_bwd_csum_kernel(const GnArgs p) {
+  constexpr int W = 8, J = GN_CT / W;
+  __shared__ float sa[GN_CT], sb[GN_CT];
+  const int tid = threadIdx.x, n = blockIdx.y, w = tid % W, c = blockIdx.x * W + w;
+  float a = 0.f, b = 0.f;
+  if (c < p.C) {
+#pragma unroll 8
+    for (int k = tid / W; k < p.chunks; k += J) {
+      const float2 s = *reinterpret_cast<const float2*>(p.part + 2 * (((long long)n * p.chunks + k) * p.C + c));
+      a += s.x;
+      b += s.y;
+    }
+  }
+  sa[tid] = a;
+  sb[tid] = b;
+  gn_sum_rows<GN_CT>(sa, W, J, tid);
+  gn_sum_rows<GN_CT>(sb, W, J, tid);
+  if (tid < W && c < p.C) *reinterpret_cast<float2*>(p.csum + 2 * ((long long)n * p.C + c)) = make_float2(sa[w], sb[w]);
+}
+__global__ __launch_bounds__(GN_CT) void gn_bwd_gsum_kernel(const GnArgs p) {
+  __shared__ float sa[GN_CT], sb[GN_CT];
+  const int tid = threadIdx.x, n = blockIdx.y, g = blockIdx.x;
+  float ta = 0.f, tb = 0.f;
+  for (int i = tid; i < p.Cg; i += GN_CT) {
+    const int c = g * p.Cg + i;
+    const float2 s = *reinterpret_cast<const float2*>(p.csum + 2 * ((long long)n * p.C + c));
+    if (p.N == 1) gn_channel_out(p, n, c, s.x, s.y);
+    const float ga = p.gamma ? p.gamma[c] : 1.f;
+    ta += s.x * ga;
+    tb += s.y * ga;
+  }
+  sa[tid] = ta;
+  sb[tid] = tb;
+  gn_sum_rows<GN_CT>(sa, 1, GN_CT, tid);
+  gn_sum_rows<GN_CT>(sb, 1, GN_CT, tid);
+  if (tid == 0) {
+    const float inv = 1.f / ((float)p.P * (float)p.Cg);
+    *reinterpret_cast<float2*>(p.gsum + 2 * ((long long)n * p.G + g)) = make_float2(sa[0] * inv, sb[0] * inv);
+  }
+}
+
 // dgamma / dbeta of channel c from the samples' sums, in sample order
 __device__ __forceinline__ void gn_param_grad(const GnArgs& p, int c) {
   if (c >= p.C) return;
@@ -912,7 +959,12 @@ template <typename T, int V> static int gn_run(const GnArgs& a, const GnPlan& pl
     } else {
       TRACE_LDS_OPT_IN((gn_bwd_sums_kernel<T, V>), 2 * GN_MAX_C * 4 + 4096, "group_norm backward");
       gn_bwd_sums_kernel<T, V><<<grid, GN_CT, lds_s, st>>>(a);
-      gn_bwd_merge_kernel<<<dim3(a.G, a.N), GN_CT, 0, st>>>(a);
+      if (pl.chunks > GN_LIST * (a.Cg >= GN_CT ? 1 : GN_CT / a.Cg)) {
+        gn_bwd_csum_kernel<<<dim3(ceil_div(a.C, 8), a.N), GN_CT, 0, st>>>(a);
+        gn_bwd_gsum_kernel<<<dim3(a.G, a.N), GN_CT, 0, st>>>(a);
+      } else {
+        gn_bwd_merge_kernel<<<dim3(a.G, a.N), GN_CT, 0, st>>>(a);
+      }
       const int extra = a.N > 1 && (a.dgamma || a.dbeta) ? ceil_div(a.C, GN_CT) : 0;
       gn_bwd_apply_kernel<T, V><<<dim3(pl.chunks + extra, a.N), GN_CT, 0, st>>>(a);
     }
