@@ -103,3 +103,28 @@ def test_captured_training_steps():
         with torch.no_grad():
             assert torch.equal(after, other.run(x))
     assert not torch.equal(seen[0][0], seen[2][0])
+
+
+def test_frozen_stages_keep_their_folded_copies():
+    """train() in every step costs no folding of what is not trained; a network that is thawed is folded again"""
+    from trace_amd.resnet3d import ResNet3d, i3d_dc5_config
+    cfg = dict(i3d_dc5_config(), norm_cfg=dict(type='GN', num_groups=32), frozen_stages=1)
+    cfg["non_local_cfg"] = dict(cfg["non_local_cfg"], norm_cfg=cfg["norm_cfg"])
+    torch.manual_seed(0)
+    m = ResNet3d(**cfg).to(DEV)
+    clip = torch.randn((1, 3, 8, 64, 64), device=DEV) * 50
+    m.eval()
+    m.forward_ndhwc(clip)
+    frozen, live = m.layer1[0].conv2, m.layer2[0].conv2
+    assert live._packed is not None
+    m.train()
+    m.forward_train(clip)
+    assert live._packed is None
+    kept = frozen.packed()[0]
+    for _ in range(2):
+        m.train()
+        m.forward_train(clip)
+        assert frozen.packed()[0] is kept and live._packed is None
+    m.frozen_stages = 0
+    m.train()
+    assert frozen._packed is None

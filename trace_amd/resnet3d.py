@@ -81,8 +81,10 @@ class ConvModule(nn.Module):
             self._packed = None
             _PACK_EPOCH[0] += 1
 
+    frozen = False   # set by ResNet3d.train: in a stage that is not trained
+
     def train(self, mode=True):
-        if mode:      # also for captured training steps, whose replays run no Python
+        if mode and not self.training and not self.frozen:      # also for captured training steps, whose replays run no Python
             self._drop_folded()
         return super().train(mode)
 
@@ -782,6 +784,10 @@ class ResNet3d(nn.Module):
 
     def train(self, mode=True):
         """resnet3d.py:804-811 (returns None like the reference)."""
+        for i, name in enumerate(['conv1'] + self.res_layers):
+            for m in getattr(self, name).modules():
+                if isinstance(m, ConvModule):
+                    m.frozen = i <= self.frozen_stages
         super().train(mode)
         if self.frozen_stages >= 0:
             self.conv1.eval()
