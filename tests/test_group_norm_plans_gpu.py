@@ -43,8 +43,11 @@ def sums(shape, G, elem, backward):
         # by side, channels of the group, a thread's list of chunks, lanes and waves
         return "two passes", 8 + 4 * (rows // unit + log2(RP) + log2(Cg) + math.ceil(chunks / 256) + 6 + 3)
     J = 1 if Cg >= 256 else 256 // Cg
-    # a thread's rows, rows side by side, a list of chunks, the lists, then the group's channels or the samples
-    return "two passes", rows // RP + log2(RP) + math.ceil(chunks / J) + log2(J) + max(math.ceil(Cg / (256 // J)) + 8, N)
+    last = max(math.ceil(Cg / (256 // J)) + 8, N)                          # the group's channels, or the samples
+    if math.ceil(chunks / J) > 64:
+        J, last = 32, max(math.ceil(Cg / 256) + 8, N)
+    # a thread's rows, rows side by side, a list of chunks, the lists
+    return "two passes", rows // RP + log2(RP) + math.ceil(chunks / J) + log2(J) + last
 
 
 CASES = [((1, 2000, 256), 4, "slab", "two passes"), ((1, 6000, 2048), 1, "two passes", "two passes"), ((1, 6000, 2048), 8, "two passes", "two passes"),
