@@ -559,7 +559,8 @@ int trace_upload_slots(const void* pinned, size_t slot_bytes, unsigned* counter,
  *            Operand rows behind q_len / kv_len are never read; rows of dk / dv behind kv_len and of dq behind q_len are
  *            written as zeros.  Keys and values in front of kv_len have to be finite also where `causal` hides them, and for the
  *            backward pass q and dout in front of q_len also in rows that see no key.
- * Nothing is summed by atomics: equal calls give equal bits.  workspace: trace_attention_{fwd,bwd}_workspace_bytes(desc)
+ * Nothing is summed by atomics: equal calls give equal bits (out with and without out_rest are two roundings of the same value: the
+ * last bit may differ).  workspace: trace_attention_{fwd,bwd}_workspace_bytes(desc)
  * bytes, 256-aligned (0: may be NULL); it is free again when the call's work on `stream` has ended. */
 typedef struct {
   int batch, q_rows, k_rows, heads, kv_heads, head_dim;
@@ -582,9 +583,10 @@ int trace_attention_bwd_bf16(const trace_attention_desc* desc, const uint16_t* q
 /* Group normalisation + activation over channels-last maps x (N, P, C), P = product of the positions, contiguous:
  *   z = (x - mean) / sqrt(var + eps) * gamma + beta with the mean / biased variance of each sample's groups of C / G
  *   channels, y = act(z); act = 0 | TRACE_EPI_RELU | TRACE_EPI_LEAKY | TRACE_EPI_SILU.  gamma / beta (C) f32, NULL = 1 / 0.
- *   stats (N, G, 2) f32: mean and 1 / sqrt(var + eps), written by the forward call, read by the backward one (of samples without positions: 0 and
- *   1 / sqrt(eps)).
+ *   stats (N, G, 2) f32: mean and 1 / sqrt(var + eps), written by the forward call, read by the backward one (of samples without
+ *   positions: 0 and 1 / sqrt(eps)).
  *   backward: dx like x, dgamma / dbeta (C) f32 (each may be NULL).
+ * N <= 65535, C <= 8192, P < 2^30.
  * workspace: trace_group_norm_workspace_bytes(N, P, C, G, backward) bytes, 256-aligned.  Sums in f32 in a fixed order. */
 size_t trace_group_norm_workspace_bytes(int N, long long P, int C, int G, int backward);
 int trace_group_norm_act_bf16(const uint16_t* x, int N, long long P, int C, int G, const float* gamma, const float* beta,

@@ -188,7 +188,8 @@ class _Attention(torch.autograd.Function):
 def attention(q, k, v, scale=None, causal=False, q_len=None, kv_len=None):
     """Differentiable ops.attention (same arguments); gradients reach q, k and v.  Kept for the backward pass: the operands,
     the output, what its rounding lost (another bf16 tensor like it) and one f32 per row - the probabilities are recomputed.
-    Without a gradient to come it is ops.attention itself."""
+    Without a gradient to come it is ops.attention itself, whose output may differ in its last bit from the one that a gradient
+    belongs to (the first pass of a checkpointed block, validation): both are within their rounding of the exact one."""
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         return ops.attention(q, k, v, scale, causal, q_len, kv_len)
     return _Attention.apply(q, k, v, scale, bool(causal), q_len, kv_len)

@@ -17,12 +17,16 @@
 // behind head_dim read a zero page, so nothing behind a length is ever touched.
 //
 // What bounds them at full size is the matrix pipe together with the vector work between its products (an exponential, its
-// scaling and its rounding per score): 2 x 4096 x 16 heads x 128 without a mask runs forward at 900 TFLOP/s, forward for a
-// backward pass at 1070 and backward at 1170 TFLOP/s of the products it executes, where a library matmul of 8192^3 reaches
-// 1190.  LDS reads take 16 % of the cycles there and conflicts none.  Three choices made that rate:
+// scaling and its rounding per score): 2 x 4096 x 16 heads x 128 without a mask runs forward at 910 - 960 TFLOP/s, forward for a
+// backward pass at 1050 - 1110 and backward at 1140 - 1200 TFLOP/s of the products it executes (calls back to back on two cards),
+// where a library matmul of 8192^3 reaches 1330.  Of the cycles that its CUs are busy, the causal one of 4 key heads spends 48 % in
+// the matrix pipe and 18 % in LDS reads (forward for a backward pass; dq 52 and 26 %, dk / dv 52 and 36 %), the forward pass of head
+// size 256 (8 x 3136 x 784) 23 % and 25 %: neither bounds it, a workgroup of four waves alone on a CU, as half of them are, has gaps that
+// nothing fills.  LDS bank conflicts: none.
+// "a -> b" below are the two sides of a choice, on one card.  Choices that made the rate:
 //   * every kernel is compiled for two waves per SIMD (256 registers): with more, hipcc keeps the sums in accumulation
-//     registers and spends hundreds of moves per tile on them (dk / dv 1173 us -> 563 us), and a single spilled register
-//     in the loop waits for the prefetch behind it (563 -> 358 us without);
+//     registers and spends hundreds of moves per tile on them (dk / dv took twice as long), and a single spilled register
+//     in the loop waits for the prefetch behind it (half as long again);
 //   * 32 columns (queries, or keys) per wave where the sums fit, so a fragment from LDS feeds two products; at head_dim 256
 //     and above 16 columns with the whole row in one wave beat 32 with the row shared by two, whose scores have to meet
 //     in LDS (8 x 3136 x 784 x 256: 60 -> 42 us), and 32 columns with the whole row spill or leave one wave
@@ -173,7 +177,7 @@ __device__ __forceinline__ at_f4 at_mfma(const at_s8& a, const at_s8& b, const a
 // Workgroups go to the 8 XCDs round-robin and each XCD has its own L2: XCD x gets the x-th contiguous eighth of the
 // (head, split, tile) units, so the tiles that read one head's other operand share an L2.  `uneven`: under a causal mask a
 // tile's work falls with its index (the caller counts from the longest); tile 0 of all heads and splits goes first then, so that
-// short ones fill the end: 2 x 4096 x 16 heads x 128, forward 211 -> 166 us, backward 566 -> 455 us.
+// short ones fill the end: 2 x 4096 x 16 heads x 128, forward 197 -> 176 us, backward 560 -> 448 us (4 key heads: 192 -> 159, 580 -> 470).
 // `spread`: single row tiles share nothing; their splits go round all XCDs, or a long batch entry would keep one of them busy alone.
 struct AtUnit {
   int tile, split, head;   // head: of all batches
@@ -216,8 +220,8 @@ template <bool FINE> __device__ __forceinline__ void at_store_out(const AttnArgs
 }
 
 // Fragments are read AT_AHEAD ahead of the products that take them: an LDS read takes longer than the NT products of one
-// fragment, and left alone hipcc reads each one right in front of its use (one ahead in hipcc's own order: 2 x 4096 x 16 heads x
-// 128 forward 355 -> 363 us, backward 821 -> 836, 8 x 3136 x 784 x 256 41 -> 45; two or six ahead as four).
+// fragment, and left alone hipcc reads each one right in front of its use (one ahead -> four: 2 x 4096 x 16 heads x 128 forward
+// 295 -> 285 us, backward 821 -> 802, 8 x 3136 x 784 x 256 46 -> 42; two or six ahead within 2 % of four).
 constexpr int AT_AHEAD = 4;
 __device__ __forceinline__ void at_order() { __builtin_amdgcn_sched_barrier(0); }
 
@@ -550,11 +554,12 @@ template <bool FINE> __global__ __launch_bounds__(256) void attn_combine_few_ker
 // dq (and delta).  The same walk as the forward's over key tiles of 32, with two scoring products (q k^T and dout v^T); the
 // second one starts from -delta instead of zero.  dS is rounded to bf16 for the product, as P is in the forward kernel.  dq and
 // dk / dv each form P and dS for themselves: seven products instead of the five of one pass, whose dq (or dk, dv) would have to
-// be added up by atomics in whatever order workgroups come.  2 x 4096 x 16 heads x 128, causal: 221 us, dk / dv 299 us.
+// be added up by atomics in whatever order workgroups come.  2 x 4096 x 16 / 4 heads x 128, causal (kernel times): 201 us, dk / dv 267 us
+// and 23 us for joining its splits.
 // The rows of dS sum to zero, so dq only has what the keys differ by, but the rounding of dS goes with all of a key: with few
 // columns the weighted mean of the keys is a good part of them (|k|^2 of D + 4 against D + 1 for unit normal q, k), and dq is
 // less exact than its own rounding explains.  Up to 32 columns a second product therefore adds what that rounding lost
-// (relative error at 8 columns 2.56e-3 -> 1.65e-3, at 16 2.48e-3 -> 1.67e-3; 4 x 2048 x 16 heads x 32: backward 170 -> 195 us).
+// (relative error at 8 columns 2.56e-3 -> 1.65e-3, at 16 2.48e-3 -> 1.67e-3; 4 x 2048 x 16 heads x 32: backward 155 -> 178 us).
 // ---------------------------------------------------------------------------------------------------------------
 template <int D, int NT, int NW, int DW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p) {
@@ -732,6 +737,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_q_kernel(const AttnArgs p
 // ---------------------------------------------------------------------------------------------------------------
 // dk and dv.  A workgroup owns NW / DW * NT * 16 keys of one (batch, key head) - in registers as B operands - and walks the
 // 32-row tiles of q and dout of every query head that reads it, so the gradients of shared heads are summed in a fixed order.
+// P and dS are rounded to bf16 for their products, at every head size: each is as much as the result's own rounding, so that dk and
+// dv are off by sqrt(2) of that (relative 2.34e-3, 1.66e-3 for the correctly rounded result; dq above 32 columns likewise).  What the
+// rounding loses would take two products more, nine for seven of the backward pass.
 // ---------------------------------------------------------------------------------------------------------------
 template <int D, int NT, int NW, int DW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_bwd_kv_kernel(const AttnArgs p) {
@@ -937,8 +945,8 @@ struct AttnPlan {
 static inline size_t at_align(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Splits so that about `per_cu` workgroups per CU exist, each with at least `min_iters` iterations of its loop (32 rows): the
-// partial results cost a pass over f32 copies of the output and a launch.  4 x 500 x 4 heads x 128: forward 18.9 us with at least
-// 8, 21.3 with 4, 25.9 with 2; backward 46.3 with 4, 50.0 with 8, 57.4 with 2.  At most `per_cu` each, or a few of them would run
+// partial results cost a pass over f32 copies of the output and a launch.  4 x 500 x 4 heads x 128: forward 17.5 us with at least
+// 8, 20.6 with 4; backward 43 with 4, 8 % more with 8, 24 % more with 2.  At most `per_cu` each, or a few of them would run
 // alone at the end (1 x 3136 x 784 x 512, backward: 13 key tiles in 20 shares 122 us, in 17 78 us), and no empty shares.
 static int at_splits(long long groups, int iters, int min_iters, int per_cu) {
   if (groups <= 0 || iters <= 0) return 1;
@@ -953,8 +961,8 @@ static int at_splits(long long groups, int iters, int min_iters, int per_cu) {
 
 // Whether half a tile of rows serves a call better than a whole one: where whole tiles would have to be split to fill the card and
 // their shares stay short (`most` iterations), the joining of the shares costs more than half tiles, whose fragments from LDS feed
-// half the products.  Forward / backward, whole against half: 128 x 8 heads causal, 8 x 1024: 54 -> 35 us / 155 -> 95, 16 x 512: 46 ->
-// 25 / 133 -> 66; 4 x 1024: 39 -> 30 / 99 -> 89; 16 x 197 x 12 heads x 64: bwd 32 -> 29; 8 x 500 x 4 heads x 256: bwd 81 -> 62.  Longer
+// half the products.  Forward / backward, whole -> half: 128 x 8 heads causal, 8 x 1024: 54 -> 34 us / 152 -> 90, 16 x 512: 45 ->
+// 23 / 130 -> 63; 4 x 1024: 39 -> 33 / 117 -> 80; 8 x 500 x 4 heads x 256: backward 80 -> 61.  Longer
 // shares (1 x 4096 x 8 heads x 128: 64 iterations): 103 -> 112 / 251 -> 296; full grids (8 x 1024): 46 -> 54 / 129 -> 157.
 static bool at_short(long long groups, int iters, int min_iters, int per_cu, int most) {
   return 2 * groups <= per_cu * AT_CUS && ceil_div(iters, at_splits(groups, iters, min_iters, per_cu)) <= most;

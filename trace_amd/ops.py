@@ -1023,7 +1023,9 @@ def attention(q, k, v, scale=None, causal=False, q_len=None, kv_len=None, return
     strided (views of a packed projection are taken as they are, other layouts are copied).  Keys and values in front of
     kv_len must be finite, also those that `causal` hides from some rows; for the backward pass so must q and dout in front of q_len.
     return_lse: -> (out, lse), lse (B,H,Nq) f32 the log-sum-exp of each row's scaled scores, -inf where it sees no key.
-    for_backward: -> (out, lse, rest), what `attention_backward` takes; rest is a second tensor like out, what rounding lost."""
+    for_backward: -> (out, lse, rest), what `attention_backward` takes; rest is a second tensor like out, what rounding lost.  The
+    probabilities are carried to 16 bits more then, so out may differ in its last bit from a call without it.
+    At most 2^30 rows; B * H * Nq and B * Hkv * Nk stay below 2^31."""
     q, k, v = _attn_operand(q, "q"), _attn_operand(k, "k"), _attn_operand(v, "v")
     B, Nq, H, D = q.shape
     dev = q.device
@@ -1105,7 +1107,7 @@ def _gn_workspace(N, P, C, G, backward):
 def group_norm_act(x, groups, gamma=None, beta=None, eps=1e-5, act=None, return_stats=False):
     """act(GroupNorm(x)) over channels-last maps x (N, ..., C), bf16 or f32 -> the same shape and type.  The statistics of a
     sample's groups of C / groups neighbouring channels run over all positions between N and C; gamma / beta (C) f32 or None;
-    act None | "relu" | "leaky" (0.1) | "silu".  With return_stats also (N, groups, 2) f32: mean and 1 / sqrt(var + eps), what
+    act None | "relu" | "leaky" (0.1) | "silu".  N <= 65535, C <= 8192.  With return_stats also (N, groups, 2) f32: mean and 1 / sqrt(var + eps), what
     `group_norm_act_backward` takes."""
     x = _map(x, "group_norm_act: x")
     N, P, C, groups, gamma, beta = _gn_args(x, groups, gamma, beta, act, "group_norm_act")

@@ -31,7 +31,8 @@ class ConvModule(nn.Module):
     """mmcv.cnn.ConvModule subset used by resnet3d.py: conv -> bn -> ReLU.
     bias='auto' means "bias iff no norm" (mmcv semantics).  norm_cfg=dict(type='GN', num_groups=..) (mmcv's name for it; eps and
     requires_grad as there) takes nn.GroupNorm as `gn` instead of the BatchNorm `bn`: its statistics belong to one clip, so it
-    trains at any batch size, but it cannot be folded into the weights."""
+    trains at any batch size, but it cannot be folded into the weights, and what a convolution's epilogue does behind a BatchNorm -
+    adding the residual, the ReLU on the sum, pool2 - are passes of their own (torch's add and ReLU, ops.maxpool3d)."""
 
     def __init__(self, in_channels, out_channels, kernel_size, stride=1, padding=0, dilation=1, bias='auto',
                  conv_cfg=None, norm_cfg=None, act_cfg=dict(type='ReLU')):
@@ -194,7 +195,8 @@ class NonLocal3d(nn.Module):
     mode='dot_product', BN on conv_out).  Source not vendored in the reference:
     restated from mmcv's published behaviour (parity unpinned).
     mode='embedded_gaussian' (mmcv's default) is softmax attention of every position over the (pooled) positions, with
-    use_scale divided by sqrt(inter_channels); it runs on ops.attention and needs inter_channels % 8 == 0, <= 512."""
+    use_scale divided by sqrt(inter_channels); `run` and `run_train` are ops.attention and take inter_channels % 8 == 0, <= 512
+    (others are refused by the call; the torch path `forward` takes any)."""
 
     def __init__(self, in_channels, reduction=2, use_scale=True, conv_cfg=None, norm_cfg=None,
                  mode='embedded_gaussian', sub_sample=False, **kwargs):
