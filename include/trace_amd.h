@@ -547,7 +547,7 @@ int trace_upload_slots(const void* pinned, size_t slot_bytes, unsigned* counter,
  * lib/i3d/resnet3d.py:289, is one head of it).  bf16 operands, f32 scores / statistics / sums.
  *   q, out, dout, dq  (batch, q_rows, heads, head_dim);  k, v, dk, dv  (batch, k_rows, kv_heads, head_dim)
  *   heads % kv_heads == 0: query head h reads key head h / (heads / kv_heads);  head_dim % 8 == 0, 8 .. 512
- *   q_rows, k_rows <= 2^30;  batch * heads * (q_rows + 2) and batch * kv_heads * (k_rows + 2) < 2^31 - 1
+ *   q_rows, k_rows <= 2^31 - 512;  batch * heads * (q_rows + 2) and batch * kv_heads * (k_rows + 2) < 2^31 - 1
  *   stride_*[3]   elements between batches / rows / heads of q, k, v (and dout), multiples of 8 (0 = broadcast); the
  *                 last dimension is contiguous, rows are 16-byte aligned.  out, dq, dk, dv are contiguous.
  *   q_len, kv_len int32 DEVICE arrays (batch) or NULL = all rows; values are clamped to 0 .. q_rows / k_rows

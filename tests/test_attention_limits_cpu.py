@@ -15,7 +15,7 @@ def desc(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(k_rows=(1 << 31) - 10), dict(q_rows=(1 << 31) - 10), dict(q_rows=(1 << 31) - 200),
-                                dict(k_rows=(1 << 30) + 1), dict(q_rows=(1 << 30) + 1)])
+                                dict(k_rows=(1 << 31) - 511), dict(q_rows=(1 << 31) - 511)])
 def test_rows_whose_tiles_pass_32_bits_are_refused(kw):
     """the last tile of 2^31 - 10 rows ends behind 2^31: row numbers would wrap to negative ones, in front of the operand"""
     from trace_amd import _lib as L
@@ -37,7 +37,8 @@ def test_grids_past_32_bits_are_refused(kw):
     assert L.lib().trace_attention_bwd_bf16(d, *[None] * 11, 0, None) != 0 and b"too many rows" in L.lib().trace_last_error()
 
 
-@pytest.mark.parametrize("kw", [dict(batch=128, heads=64, kv_heads=8, q_rows=1, k_rows=262144, head_dim=128), dict(heads=8, kv_heads=1, k_rows=1 << 30),
+@pytest.mark.parametrize("kw", [dict(batch=128, heads=64, kv_heads=8, q_rows=1, k_rows=262144, head_dim=128), dict(heads=8, kv_heads=1, k_rows=(1 << 31) - 512),
+                                dict(q_rows=(1 << 31) - 512, k_rows=1),
                                 dict(batch=1 << 12, heads=1 << 9, q_rows=1, k_rows=1 << 16)])
 def test_query_heads_times_key_rows_is_no_limit(kw):
     """the call passes the check of its sizes: the next thing that is wrong with it, null pointers, is what it is refused for"""

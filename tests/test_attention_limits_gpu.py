@@ -50,3 +50,20 @@ def test_rows_are_counted_apart():
     # of P and one of the result
     assert not dq.any() and float(dk.float().abs().max()) <= H * D ** -0.5 / Nk * 8 * 4 * F
     assert float((dv.float() * (Nk / 64.0) - 1).abs().max()) <= 2 * U + U * U + 1e-5
+
+
+def test_rows_past_30_bits():
+    """1.5 x 2^30 keys, all of them one row in memory: the mean of equal values, the logarithm of their number and, under a causal
+    mask, the same (the last query sees every key)"""
+    from trace_amd import ops
+    Nk, D = 3 << 29, 8
+    q = torch.full((1, 1, 1, D), 0.5, dtype=torch.bfloat16, device=DEV)
+    k = torch.full((1, 1, 1, D), 0.25, dtype=torch.bfloat16, device=DEV).expand(1, Nk, 1, D)
+    v = torch.arange(D, device=DEV).to(torch.bfloat16).view(1, 1, 1, D).expand(1, Nk, 1, D)
+    for causal in (False, True):
+        out, lse = ops.attention(q, k, v, causal=causal, return_lse=True)
+        assert torch.equal(out, v[:, :1])
+        want = D * 0.125 * D ** -0.5 + math.log(Nk)
+        assert abs(float(lse) - want) <= 8 * 2.0 ** -23 * want
+    few = torch.tensor([Nk - 7], dtype=torch.int32, device=DEV)
+    assert torch.equal(ops.attention(q, k, v, kv_len=few), v[:, :1])

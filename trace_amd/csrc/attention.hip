@@ -46,7 +46,7 @@ __device__ __attribute__((aligned(256))) const uint4 g_at_zero[16] = {};
 constexpr float AT_LOG2E = 1.4426950408889634f, AT_LN2 = 0.6931471805599453f;
 constexpr int AT_CUS = 256;
 constexpr int AT_MAX_SPLITS = 256;   // a thread each in attn_combine_kernel
-constexpr int AT_MAX_ROWS = 1 << 30;
+constexpr int AT_MAX_ROWS = 0x7fffffff - 511;
 
 struct AttnArgs {
   const uint16_t *q, *k, *v, *out, *rest, *dout;
@@ -1017,8 +1017,8 @@ static int at_check(const trace_attention_desc* d, const char* what) {
   TRACE_REQUIRE(d->head_dim >= 8 && d->head_dim <= 512 && d->head_dim % 8 == 0, "%s: head_dim %d (8 .. 512, multiple of 8)",
                 what, d->head_dim);
   TRACE_REQUIRE(d->scale > 0.f && d->scale <= 3.0e38f, "%s: scale must be positive and finite", what);
-  // rows are counted in 32 bits to the end of the last tile, and a causal mask adds q_rows to k_rows
-  TRACE_REQUIRE(d->q_rows <= AT_MAX_ROWS && d->k_rows <= AT_MAX_ROWS, "%s: too many rows (at most 2^30)", what);
+  // rows are counted in 32 bits to the end of the last tile (at most 128 rows) and one tile further
+  TRACE_REQUIRE(d->q_rows <= AT_MAX_ROWS && d->k_rows <= AT_MAX_ROWS, "%s: too many rows (at most 2^31 - 512)", what);
   // tiles x heads x batch are grid indices, of query heads over query rows (rows x heads of a packed call are row indices too) and
   // of key heads over key rows
   const long long qr = (long long)d->batch * d->heads * (d->q_rows + 2), kr = (long long)d->batch * d->kv_heads * (d->k_rows + 2);

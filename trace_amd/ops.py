@@ -1025,7 +1025,7 @@ def attention(q, k, v, scale=None, causal=False, q_len=None, kv_len=None, return
     return_lse: -> (out, lse), lse (B,H,Nq) f32 the log-sum-exp of each row's scaled scores, -inf where it sees no key.
     for_backward: -> (out, lse, rest), what `attention_backward` takes; rest is a second tensor like out, what rounding lost.  The
     probabilities are carried to 16 bits more then, so out may differ in its last bit from a call without it.
-    At most 2^30 rows; B * H * Nq and B * Hkv * Nk stay below 2^31."""
+    At most 2^31 - 512 rows; B * H * Nq and B * Hkv * Nk stay below 2^31."""
     q, k, v = _attn_operand(q, "q"), _attn_operand(k, "k"), _attn_operand(v, "v")
     B, Nq, H, D = q.shape
     dev = q.device
