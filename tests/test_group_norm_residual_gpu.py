@@ -49,6 +49,23 @@ def test_bottleneck_keeps_the_sum_in_f32(down):
     assert e32 < 2.0 ** -8 and e32 < e16, (e32, e16)
 
 
+@pytest.mark.parametrize("main,side", [("GN", "BN"), ("BN", "GN")])
+def test_bottleneck_of_both_norms(main, side):
+    """a block whose downsample has the other norm: the f32 sum rounds to what the bf16 stream gives, but for that stream's roundings"""
+    from trace_amd.resnet3d import Bottleneck3d, ConvModule
+    torch.manual_seed(9)
+    cfg = {"GN": CFG, "BN": dict(type='BN3d')}
+    blk = Bottleneck3d(64, 32, downsample=ConvModule(64, 128, 1, bias=False, norm_cfg=cfg[side], act_cfg=None), norm_cfg=cfg[main]).eval().to(DEV)
+    x = torch.randn((2, 2, 6, 6, 64), device=DEV).bfloat16()
+    with torch.no_grad():
+        plain = blk.run(x)
+        blk.res_f32 = True
+        out = blk.run(x)
+    assert torch.equal(out._res32.bfloat16(), out)
+    # the plain stream rounds both branches, the convolution under a GroupNorm and the sum: four roundings of u / sqrt(3) each
+    assert rel(plain, out._res32) < 4 * 2.0 ** -8 / 3 ** 0.5
+
+
 @pytest.mark.parametrize("mode", ["embedded_gaussian", "dot_product"])
 @pytest.mark.parametrize("sub", [False, True])
 def test_nonlocal_keeps_the_sum_in_f32(mode, sub):

@@ -419,7 +419,7 @@ class Bottleneck3d(nn.Module):
             else:
                 identity = x32 if x32 is not None else x.float()
             h = self.conv2.run(self.conv1.run(x))
-            if gn:
+            if self.conv3.with_gn:
                 out = self.conv3.run_f32(h, identity, True)
                 return self.non_local_block.run(out) if self.non_local else out
             w3, b3 = self.conv3.packed()
